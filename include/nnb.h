@@ -408,6 +408,31 @@ NNB_API nnb_status nnb_step_advance(void* stream, int64_t* step);
  * Same arithmetic, same bits. */
 NNB_API nnb_status nnb_adamw_step_device(void* stream, size_t n, float* w, const float* g, float* m, float* v,
 		const float* hyper, const float* bias_table, size_t table_len, const int64_t* step);
+/* One AdamW step over `count` parameters in one launch (Adam::step's loop over its parameters,
+ * src/optim/adam.cpp:28-43): tensor i has n[i] elements at w[i], g[i], m[i], v[i] (host arrays of
+ * device pointers, read before the call returns; n[i] == 0 skips it, g[i] == NULL is a gradient of
+ * zeros). The tensors must not overlap. Bitwise nnb_adamw_step on each; no alignment is required (16
+ * bytes run fastest). Lists above 480 tensors take one launch per 480. */
+NNB_API nnb_status nnb_adamw_multi_step(void* stream, size_t count, const size_t* n, float* const* w,
+		const float* const* g, float* const* m, float* const* v, float lr, float beta1, float beta2, float eps,
+		float weight_decay, long long step);
+/* The same with both moments in 8 bits (no reference counterpart: nn-cpp's optimizers keep fp32). Every
+ * NNB_ADAMW8_BLOCK consecutive elements of a tensor (fewer at its end) share one unit per moment,
+ * m_unit[i] and v_unit[i] holding ceil(n[i] / NNB_ADAMW8_BLOCK) floats each: a code k of m (signed)
+ * stands for sign(k) k^2 unit, a code k of v (unsigned) for (k^2 unit)^2 -- v's codes hold its root.
+ * After the step unit = max|m| / 127^2 (or max sqrt(v) / 255^2) over the block and each code is the
+ * nearest, a root above zero getting at least 1; a block whose largest value is below 2^-100 is
+ * stored as zeros. The update itself uses the unrounded new moments:
+ * w = w (1 - lr wd) - (lr / (1 - beta1^t)) m / (sqrt(v) / sqrt(1 - beta2^t) + eps). All codes and units
+ * zero is the state before the first step. A gradient that is not finite makes its whole block's state
+ * NaN (in 32 bits: its element's). */
+#define NNB_ADAMW8_BLOCK 256
+NNB_API nnb_status nnb_adamw8_multi_step(void* stream, size_t count, const size_t* n, float* const* w,
+		const float* const* g, int8_t* const* m, uint8_t* const* v, float* const* m_unit, float* const* v_unit, float lr,
+		float beta1, float beta2, float eps, float weight_decay, long long step);
+/* The moments that the codes of one tensor stand for, as fp32. */
+NNB_API nnb_status nnb_adamw8_moments(void* stream, size_t n, const int8_t* m, const uint8_t* v, const float* m_unit,
+		const float* v_unit, float* m_out, float* v_out);
 
 /*
  * nnb_sgemm_ex for callers that cannot allocate device memory. This entry point has no

@@ -437,34 +437,110 @@ class Sequential(Module):
         return out
 
 
+def _addresses(who: str, tensors, sizes) -> list[int]:
+    """The device addresses of contiguous fp32 buffers of the given sizes on the current CUDA device; any
+    other tensor is refused (its pointer would reach the kernels unchecked)."""
+    out, dev, f32 = [], torch.cuda.current_device(), torch.float32
+    for t, n in zip(tensors, sizes):
+        if t.get_device() != dev:
+            raise ValueError(f"{who}: tensors must be on the current CUDA device, one is on {t.device}")
+        if t.dtype is not f32 or not t.is_contiguous():
+            raise ValueError(f"{who}: tensors must be contiguous float32")
+        if t.numel() != n:
+            raise TensorShapeError(f"{who}: a parameter or its gradient changed its size")
+        out.append(t.data_ptr())
+    return out
+
+
+def _pointers(addresses):
+    return (ctypes.c_void_p * len(addresses))(*addresses)
+
+
 class AdamW:
     """Decoupled weight decay then Adam (src/optim/adamw.cpp:15-24, src/optim/adam.cpp:24-43), one
-    fused kernel per parameter; the moment buffers start at zero."""
+    launch for the whole parameter list; the moments start at zero.
 
-    def __init__(self, params, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2):
+    state_bits=8 keeps both moments as 8-bit codes with one fp32 unit per 256 elements
+    (nnb_adamw8_multi_step, include/nnb.h): 2 bytes of state per parameter instead of 8.
+
+    The states are one flat buffer each, flat_m and flat_v, parameter i's part starting at offsets[i]
+    (a whole number of 256-element blocks) with zeros behind it; m[i] and v[i] are views of the parts.
+    With 8 bits they hold the codes, and unit_m / unit_v the units, block after block."""
+
+    BLOCK = 256
+
+    def __init__(self, params, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, state_bits=32):
+        if state_bits not in (32, 8):
+            raise ValueError("AdamW: state_bits must be 32 or 8")
         self.params = list(params)
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
+        self.state_bits = state_bits
+        sizes = [p.data.numel() for p in self.params]
+        if self.params:
+            _addresses("AdamW", [p.data for p in self.params], sizes)
+        self.offsets = [0]
+        for n in sizes:
+            self.offsets.append(self.offsets[-1] + -(-n // self.BLOCK) * self.BLOCK)
+        total = self.offsets[-1]
+        dev = self.params[0].data.device if self.params else None
         s = torch.cuda.current_stream().cuda_stream
-        self.m, self.v = [], []
-        for p in self.params:
-            for buf in (self.m, self.v):
-                t = torch.empty_like(p.data)
-                check(lib().nnb_fill(s, t.numel(), 0.0, t.data_ptr()))
-                buf.append(t)
+
+        def zeros(count, dtype):
+            t = torch.empty(count, dtype=dtype, device=dev)
+            words = t.view(torch.float32)
+            check(lib().nnb_fill(s, words.numel(), 0.0, words.data_ptr()))
+            return t
+
+        kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
+        self.flat_m, self.flat_v = (zeros(total, k) for k in kinds)
+        self.m, self.v = ([flat[o: o + n].view(p.data.shape) for p, n, o in zip(self.params, sizes, self.offsets)]
+                          for flat in (self.flat_m, self.flat_v))
+        self._sizes, self._n = sizes, (ctypes.c_size_t * len(sizes))(*sizes)
+        self._states = [_pointers([t.data_ptr() for t in ts]) for ts in (self.m, self.v)]
+        if state_bits == 8:
+            self.unit_m, self.unit_v = (zeros(total // self.BLOCK, torch.float32) for _ in range(2))
+            self._states += [_pointers([u.data_ptr() + 4 * (o // self.BLOCK) for o in self.offsets[:-1]])
+                             for u in (self.unit_m, self.unit_v)]
         self.t = 0
 
     def zero_grad(self):
         for p in self.params:
             p.zero_grad()
 
+    def flat_moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """Both moments of every parameter in fp32, laid out as flat_m and flat_v are: those buffers
+        themselves with 32-bit states, new ones with the values the codes stand for with 8-bit states."""
+        if self.state_bits == 32:
+            return self.flat_m, self.flat_v
+        m, v = (torch.empty(self.offsets[-1], dtype=torch.float32, device=self.flat_m.device) for _ in range(2))
+        check(lib().nnb_adamw8_moments(torch.cuda.current_stream().cuda_stream, m.numel(), self.flat_m.data_ptr(),
+                                       self.flat_v.data_ptr(), self.unit_m.data_ptr(), self.unit_v.data_ptr(),
+                                       m.data_ptr(), v.data_ptr()))
+        return m, v
+
+    def moments(self) -> list[tuple[torch.Tensor, torch.Tensor]]:
+        """(m, v) of each parameter in its shape, views of flat_moments()."""
+        m, v = self.flat_moments()
+        return [(m[o: o + p.data.numel()].view(p.data.shape), v[o: o + p.data.numel()].view(p.data.shape))
+                for p, o in zip(self.params, self.offsets)]
+
     # -- checkpoint state (src/optim/adam.cpp:46-71; AdamW has the same entries) -------------------
     def state(self) -> list[tuple[str, torch.Tensor]]:
+        """With 8-bit states m.i and v.i are the codes, as fp32 whole numbers, and m_unit.i and v_unit.i
+        their units: loading them gives back the same codes."""
         dev = self.m[0].device if self.m else torch.device("cpu")
         out = [(n, torch.tensor([v], dtype=torch.float32, device=dev))
                for n, v in (("lr", self.lr), ("beta1", self.beta1), ("beta2", self.beta2), ("eps", self.eps),
                             ("t", float(self.t)))]
-        out += [(f"m.{i}", m) for i, m in enumerate(self.m)]
-        out += [(f"v.{i}", v) for i, v in enumerate(self.v)]
+        out += [(name, t if t.dtype == torch.float32 else t.to(torch.float32)) for name, t in self._buffers()]
+        return out
+
+    def _buffers(self) -> list[tuple[str, torch.Tensor]]:
+        out = [(f"m.{i}", m) for i, m in enumerate(self.m)] + [(f"v.{i}", v) for i, v in enumerate(self.v)]
+        if self.state_bits == 8:
+            spans = [(a // self.BLOCK, b // self.BLOCK) for a, b in zip(self.offsets, self.offsets[1:])]
+            for name, units in (("m_unit", self.unit_m), ("v_unit", self.unit_v)):
+                out += [(f"{name}.{i}", units[a:b]) for i, (a, b) in enumerate(spans)]
         return out
 
     def load_state(self, snapshot) -> None:
@@ -475,33 +551,48 @@ class AdamW:
             raise RuntimeError("optimizer state mismatch: duplicate entries")
         if "lr" not in got:
             got["lr"] = np.array([self.lr], np.float32)
-        want = self.state()
+        want = [(n, (1,)) for n in ("lr", "beta1", "beta2", "eps", "t")]
+        want += [(n, tuple(t.shape)) for n, t in self._buffers()]
         problems = ""
-        for name, t in want:
+        for name, shape in want:
             if name not in got:
                 problems += " missing:" + name
-            elif tuple(np.shape(got[name])) != tuple(t.shape):
+            elif tuple(np.shape(got[name])) != shape:
                 problems += " shape-mismatch:" + name
         names = {n for n, _ in want}
         problems += "".join(" unexpected:" + n for n in got if n not in names)
+        if not problems and self.state_bits == 8:
+            for name, t in self._buffers():
+                if t.dtype != torch.float32:
+                    codes, low = np.asarray(got[name], np.float32), -127 if t.dtype == torch.int8 else 0
+                    if not np.all((codes == np.rint(codes)) & (codes >= low) & (codes <= low + 254 + (low == 0))):
+                        problems += " not-codes:" + name
         if problems:
             raise RuntimeError("optimizer state mismatch:" + problems)
         val = lambda n: float(np.asarray(got[n], np.float32).reshape(-1)[0])
         self.lr, self.beta1, self.beta2, self.eps = val("lr"), val("beta1"), val("beta2"), val("eps")
         self.t = int(val("t"))
-        for i, (m, v) in enumerate(zip(self.m, self.v)):
-            m.copy_(torch.as_tensor(np.asarray(got[f"m.{i}"], np.float32)).to(m.device))
-            v.copy_(torch.as_tensor(np.asarray(got[f"v.{i}"], np.float32)).to(v.device))
+        for name, t in self._buffers():
+            t.copy_(torch.as_tensor(np.asarray(got[name], np.float32)).to(t.dtype).to(t.device))
 
     def step(self):
-        import ctypes
-        self.t += 1
+        if not self.params:
+            self.t += 1
+            return
         s = torch.cuda.current_stream().cuda_stream
-        for p, m, v in zip(self.params, self.m, self.v):
+        for p in self.params:
             if p.grad_fresh:     # nothing reached this parameter: its gradient is all zeros
                 check(lib().nnb_fill(s, p.grad.numel(), 0.0, p.grad.data_ptr()))
                 p.grad_fresh = False
-            check(lib().nnb_adamw_step(s, p.data.numel(), p.data.data_ptr(), p.grad.data_ptr(), m.data_ptr(),
-                                       v.data_ptr(), ctypes.c_float(self.lr), ctypes.c_float(self.beta1),
-                                       ctypes.c_float(self.beta2), ctypes.c_float(self.eps),
-                                       ctypes.c_float(self.weight_decay), self.t))
+        w = _addresses("AdamW", [p.data for p in self.params], self._sizes)
+        g = _addresses("AdamW", [p.grad for p in self.params], self._sizes)
+        update = lib().nnb_adamw_multi_step if self.state_bits == 32 else lib().nnb_adamw8_multi_step
+        scalars = (self.lr, self.beta1, self.beta2, self.eps, self.weight_decay)
+        self.t += 1
+        used = [a for a, n in zip(w, self._sizes) if n]
+        if len(set(used)) == len(used):
+            check(update(s, len(w), self._n, _pointers(w), _pointers(g), *self._states, *scalars, self.t))
+            return
+        for i in range(len(w)):      # a parameter listed twice is updated twice, one after the other
+            check(update(s, 1, (ctypes.c_size_t * 1)(self._n[i]), _pointers(w[i: i + 1]), _pointers(g[i: i + 1]),
+                         *(_pointers(ps[i: i + 1]) for ps in self._states), *scalars, self.t))

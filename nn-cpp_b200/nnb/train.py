@@ -74,6 +74,8 @@ class ShardedTrainer:
     def __init__(self, model, optimizer, shards: int = 8, world: int = 1, rank: int = 0, group=None):
         if shards % world:
             raise ValueError("the virtual shard count must be a multiple of the number of ranks")
+        if getattr(optimizer, "state_bits", 32) != 32:
+            raise ValueError("ShardedTrainer keeps 32-bit moments of its own: use an AdamW with state_bits=32")
         self.model, self.opt = model, optimizer
         self.shards, self.world, self.rank, self.group = shards, world, rank, group
         self.owned = shard_owners(shards, world, rank)
