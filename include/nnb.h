@@ -425,7 +425,7 @@ NNB_API nnb_status nnb_adamw_multi_step(void* stream, size_t count, const size_t
  * stored as zeros. The update itself uses the unrounded new moments:
  * w = w (1 - lr wd) - (lr / (1 - beta1^t)) m / (sqrt(v) / sqrt(1 - beta2^t) + eps). All codes and units
  * zero is the state before the first step. A gradient that is not finite makes its whole block's state
- * NaN (in 32 bits: its element's). */
+ * not finite (in 32 bits: its element's). */
 #define NNB_ADAMW8_BLOCK 256
 NNB_API nnb_status nnb_adamw8_multi_step(void* stream, size_t count, const size_t* n, float* const* w,
 		const float* const* g, int8_t* const* m, uint8_t* const* v, float* const* m_unit, float* const* v_unit, float lr,

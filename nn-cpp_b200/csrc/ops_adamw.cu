@@ -7,7 +7,7 @@
 //
 // 32 bits: the element operations and their order are adamw_kernel's (ops_elementwise.cu), so the
 // results are bitwise those of one nnb_adamw_step per tensor. It moves 28 bytes per element and is
-// bound by HBM.
+// bound by HBM: 558 us for 2^27 elements, 6.7 TB/s (the measured copy rate is 6.55).
 //
 // 8 bits: block-wise quantised moments in the manner of Dettmers et al. (8-bit optimizers via
 // block-wise quantization, 2022), with a code chosen for arithmetic instead of a table: 256 consecutive
@@ -28,19 +28,23 @@ namespace nnb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;             // elements per CTA: 4 float4 per thread; 16 blocks of 256
+constexpr int kThreads8 = 128;           // 8-bit states
+constexpr int kChunk = 4096;             // elements per CTA with 32-bit states: 4 float4 per thread
+constexpr int kChunk8 = kThreads8 / 32 * NNB_ADAMW8_BLOCK;   // with 8-bit states: a block per warp
 constexpr int kBlock = NNB_ADAMW8_BLOCK; // elements that share a unit: one warp, 8 per lane
 constexpr float kTiny = 0x1p-100f;       // blocks whose largest value is below this are stored as zeros
-static_assert(kBlock == 256 && kChunk % kBlock == 0, "a warp takes a block as two float4 per lane");
+static_assert(kBlock == 256 && kChunk8 % kBlock == 0, "a warp takes a block as two float4 per lane");
 
 struct Scalars {
 	float shrink, lr, b1, keep1, b2, keep2, eps, c1, c2;
+	float minus_lr_c1, inv_root_c2;       // -lr / c1 and 1 / sqrt(c2), the 8-bit form's
 };
 
 // The list of one launch. kCap tensors fit in the classic 4 KB of parameters (small launches stay
 // cheap) or in the 32 KB that sm_70 and later take.
 template <int kCap>
 struct List32 {
+	static constexpr int kPerChunk = kChunk;
 	Scalars s;
 	int count;
 	unsigned first[kCap + 1];              // first[i]: chunks before tensor i
@@ -52,6 +56,7 @@ struct List32 {
 };
 template <int kCap>
 struct List8 {
+	static constexpr int kPerChunk = kChunk8;
 	Scalars s;
 	int count;
 	unsigned first[kCap + 1];
@@ -129,26 +134,23 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
 // Value of a code: sign(k) k^2 u (k^2 is exact; one rounding).
 __device__ __forceinline__ float decode(float k, float u) { return k * fabsf(k) * u; }
 
-// The code whose square is nearest to t, ties up: k with k^2 - k + 1/2 <= t < k^2 + k + 1/2, at most
-// `levels`; 0 for a t below 1/2 or NaN. The approximate root is within one of k, and the comparisons
-// that settle it are exact (the bounds are multiples of 1/2 below 2^17), so the code does not depend
-// on the root's rounding.
-__device__ __forceinline__ float encode(float t, float levels) {
+// The code whose square is nearest to t = x inv: k with k^2 - k + 1/2 <= t < k^2 + k + 1/2; 0 for a NaN.
+// k = floor(sqrt(t - 1/4) + 1/2), and the approximate root (relative error 2^-23) of a t made smaller by
+// 2^-18 (inv_low) rounds to k or to k - 1, never above: one comparison settles it, and that is exact
+// (the bound is a multiple of 1/2 below 2^17), so the code depends on t alone, not on the root's
+// rounding. No code exceeds `levels` because the largest t is levels^2 (1 + 2^-23).
+constexpr float kRoundMagic = 12582912.0f;                  // 1.5 * 2^23: adding it rounds to whole numbers
+__device__ __forceinline__ float encode(float x, float inv, float inv_low, float& t) {
+	t = x * inv;
 	float r;
-	asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
-	const float k = rintf(r), k2 = k * k + 0.5f;
-	float o = t >= k2 + k ? k + 1.0f : t < k2 - k ? k - 1.0f : k;
-	o = fminf(o, levels);
-	return t >= 0.5f ? o : 0.0f;
+	asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(__fmaf_rn(x, inv_low, -0.25f), 0.0f)));
+	const float k = __fadd_rn(__fadd_rn(r, kRoundMagic), -kRoundMagic), up = k + 1.0f;
+	return t >= __fmaf_rn(k, up, 0.5f) ? up : k;
 }
-
-// Unit and its inverse of a block whose largest magnitude has the bit pattern `top` (as unsigned
-// integers magnitudes order as the values do, NaN above infinity: a block that holds a NaN gets a NaN
-// unit and reads back as NaN throughout, one that holds an infinity reads back as NaN and infinity).
-__device__ __forceinline__ void block_unit(unsigned top, float levels2, float& unit, float& inv) {
-	const float a = __uint_as_float(top);
-	unit = a < kTiny ? 0.0f : a / levels2;
-	inv = a < kTiny ? 0.0f : levels2 / a;
+// The low byte of a whole number in [-128, 255], two's complement.
+__device__ __forceinline__ uint32_t code_bits(float k) { return __float_as_uint(k + kRoundMagic); }
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+	return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // One block by one warp: lane l holds elements 4l .. 4l + 3 and 128 + 4l .. 128 + 4l + 3.
@@ -190,34 +192,48 @@ __device__ __forceinline__ void load_block(Block8& b, bool vec, int n, int lane,
 }
 
 // The step on a loaded block, its new units and its stores. The root r' = sqrt(v') serves both the
-// update, w - (lr / c1) m' / (r' / sqrt(c2) + eps), and the stored code.
-__device__ __forceinline__ void step_block(Block8& b, const Scalars& s, float lr_c1, float inv_root_c2, bool vec, int n,
+// update, w - (lr / c1) m' / (r' / sqrt(c2) + eps), and the stored code. The update's division is the
+// approximate one (2 ulp of a step that is small next to w).
+//
+// Units: as unsigned integers the bit patterns of magnitudes order as the values do, NaN above infinity,
+// so a block that holds a NaN or an infinity gets such a unit and reads back as not finite throughout.
+// The two units and their inverses are four correctly rounded divisions that every lane would repeat:
+// the lower half-warp works out m's pair, the upper half v's, and two shuffles hand the inverses over.
+__device__ __forceinline__ void step_block(Block8& b, const Scalars& s, bool vec, int n,
 		int lane, float* w, int8_t* m, uint8_t* v, float* mu, float* vu) {
 	float mv[8], rv[8];
 	unsigned top_m = 0, top_r = 0;
 #pragma unroll
 	for (int q = 0; q < 8; ++q) {
 		const float km = (float)(int8_t)(b.m[q >> 2] >> (8 * (q & 3))), kr = (float)(uint8_t)(b.v[q >> 2] >> (8 * (q & 3)));
-		const float r0 = decode(kr, b.vu), g = b.g[q];
+		const float r0 = kr * kr * b.vu, g = b.g[q];
 		mv[q] = s.b1 * decode(km, b.mu) + s.keep1 * g;
 		rv[q] = sqrtf(s.b2 * (r0 * r0) + s.keep2 * g * g);
-		b.w[q] = b.w[q] * s.shrink - __fdividef(lr_c1 * mv[q], rv[q] * inv_root_c2 + s.eps);
+		float rcp;
+		asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(__fmaf_rn(rv[q], s.inv_root_c2, s.eps)));
+		b.w[q] = __fmaf_rn(s.minus_lr_c1 * mv[q], rcp, b.w[q] * s.shrink);
 		top_m = max(top_m, __float_as_uint(mv[q]) & 0x7fffffffu);
 		top_r = max(top_r, __float_as_uint(rv[q]) & 0x7fffffffu);
 	}
 	top_m = __reduce_max_sync(0xffffffffu, top_m);
 	top_r = __reduce_max_sync(0xffffffffu, top_r);
-	float um, im, ur, ir;
-	block_unit(top_m, 16129.0f, um, im);
-	block_unit(top_r, 65025.0f, ur, ir);
-	b.m[0] = b.m[1] = b.v[0] = b.v[1] = 0;
+	const float top = __uint_as_float(lane < 16 ? top_m : top_r), levels2 = lane < 16 ? 16129.0f : 65025.0f;
+	const float unit = top < kTiny ? 0.0f : top / levels2, inv = top < kTiny ? 0.0f : levels2 / top;
+	const float im = __shfl_sync(0xffffffffu, inv, 0), ir = __shfl_sync(0xffffffffu, inv, 16);
+	constexpr float kLow = 1.0f - 0x1p-18f;
+	const float im_low = im * kLow, ir_low = ir * kLow;
+	uint32_t cm[8], cr[8];
 #pragma unroll
 	for (int q = 0; q < 8; ++q) {
-		const int km = (int)encode(fabsf(mv[q]) * im, 127.0f);
-		int kr = (int)encode(rv[q] * ir, 255.0f);
-		if (rv[q] > 0.0f && ur > 0.0f) kr = max(kr, 1);
-		b.m[q >> 2] |= (uint32_t)(uint8_t)(mv[q] < 0.0f ? -km : km) << (8 * (q & 3));
-		b.v[q >> 2] |= (uint32_t)kr << (8 * (q & 3));
+		float t;
+		cm[q] = code_bits(copysignf(encode(fabsf(mv[q]), im, im_low, t), mv[q]));
+		const float kr = encode(rv[q], ir, ir_low, t);
+		cr[q] = code_bits(fmaxf(kr, t > 0.0f ? 1.0f : 0.0f));
+	}
+#pragma unroll
+	for (int h = 0; h < 2; ++h) {
+		b.m[h] = pack4(cm[4 * h], cm[4 * h + 1], cm[4 * h + 2], cm[4 * h + 3]);
+		b.v[h] = pack4(cr[4 * h], cr[4 * h + 1], cr[4 * h + 2], cr[4 * h + 3]);
 	}
 	if (vec) {
 #pragma unroll
@@ -238,35 +254,33 @@ __device__ __forceinline__ void step_block(Block8& b, const Scalars& s, float lr
 			}
 		}
 	}
-	if (lane == 0) {
-		*mu = um;
-		*vu = ur;
-	}
+	// (every lane read the old units before the warp's reductions above)
+	if (lane == 0) *mu = unit;
+	if (lane == 16) *vu = unit;
 }
 
+// One block per warp, in small CTAs: 56 registers leave 36 warps on an SM, whose loads cover HBM's
+// latency and each other's arithmetic (about 70 instructions per element, two thirds of what the issue
+// slots give in the time HBM needs). 2^27 elements: 370 us, 5.8 TB/s, 0.89 of the measured copy rate.
+// Measured against it: CTAs of 256 threads 384 to 394 us; several blocks per warp, even with the next
+// block's loads issued ahead, 400 to 850 us (the warps drift apart in a long loop body).
 template <int kCap>
-__global__ void __launch_bounds__(kThreads) adamw8_multi_kernel(const __grid_constant__ List8<kCap> l) {
+__global__ void __launch_bounds__(kThreads8, 9) adamw8_multi_kernel(const __grid_constant__ List8<kCap> l) {
 	const int ti = find_tensor(l, blockIdx.x);
-	const long long base = (long long)(blockIdx.x - l.first[ti]) * kChunk;
-	const int n = (int)min((long long)kChunk, l.n[ti] - base);
+	const long long base = (long long)(blockIdx.x - l.first[ti]) * kChunk8 + (threadIdx.x >> 5) * kBlock;
+	if (base >= l.n[ti]) return;                   // warp-uniform
+	const int n = (int)min((long long)kBlock, l.n[ti] - base), lane = threadIdx.x & 31;
 	float* w = l.w[ti] + base;
 	const float* g = l.g[ti] ? l.g[ti] + base : nullptr;
 	int8_t* m = l.m[ti] + base;
 	uint8_t* v = l.v[ti] + base;
 	float* mu = l.mu[ti] + base / kBlock;
 	float* vu = l.vu[ti] + base / kBlock;
-	const Scalars& s = l.s;
-	const float lr_c1 = s.lr / s.c1, inv_root_c2 = 1.0f / sqrtf(s.c2);
-	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-	const bool aligned = ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(g)) & 15) == 0 &&
+	const bool vec = n == kBlock && ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(g)) & 15) == 0 &&
 		((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 3) == 0;
-	for (int o = warp * kBlock; o < n; o += (kThreads / 32) * kBlock) {     // warp-uniform
-		const bool vec = aligned && n - o >= kBlock;
-		Block8 b;
-		load_block(b, vec, n - o, lane, w + o, g ? g + o : nullptr, m + o, v + o, mu + o / kBlock, vu + o / kBlock);
-		__syncwarp();                          // every lane has read the units before lane 0 replaces them
-		step_block(b, s, lr_c1, inv_root_c2, vec, n - o, lane, w + o, m + o, v + o, mu + o / kBlock, vu + o / kBlock);
-	}
+	Block8 b;
+	load_block(b, vec, n, lane, w, g, m, v, mu, vu);
+	step_block(b, l.s, vec, n, lane, w, m, v, mu, vu);
 }
 
 // The moments that the codes stand for: m = sign(k) k^2 u, v = (k^2 u)^2. Four elements per thread.
@@ -313,6 +327,8 @@ Scalars host_scalars(float lr, float b1, float b2, float eps, float wd, long lon
 	s.b2 = b2;
 	s.keep2 = 1.0f - b2;
 	s.eps = eps;
+	s.minus_lr_c1 = -lr / s.c1;
+	s.inv_root_c2 = 1.0f / std::sqrt(s.c2);
 	return s;
 }
 
@@ -345,7 +361,7 @@ void launch(cudaStream_t s, unsigned chunks, const List32<kCap>& l) {
 }
 template <int kCap>
 void launch(cudaStream_t s, unsigned chunks, const List8<kCap>& l) {
-	adamw8_multi_kernel<kCap><<<chunks, kThreads, 0, s>>>(l);
+	adamw8_multi_kernel<kCap><<<chunks, kThreads8, 0, s>>>(l);
 }
 
 // Fills lists of up to kCap non-empty tensors (and 2^31 - 1 chunks) and launches each.
@@ -359,7 +375,7 @@ nnb_status run_lists(cudaStream_t s, const Scalars& sc, const Spec& a) {
 		unsigned long long chunks = 0;
 		for (; i < a.count && k < kCap; ++i) {
 			if (a.n[i] == 0) continue;
-			const unsigned long long c = (a.n[i] + kChunk - 1) / kChunk;
+			const unsigned long long c = (a.n[i] + List::kPerChunk - 1) / List::kPerChunk;
 			if (k > 0 && chunks + c > 0x7fffffffull) break;
 			l.first[k] = (unsigned)chunks;
 			l.n[k] = (long long)a.n[i];
