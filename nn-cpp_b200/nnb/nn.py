@@ -440,7 +440,8 @@ class Sequential(Module):
 def _addresses(who: str, tensors, sizes) -> list[int]:
     """The device addresses of contiguous fp32 buffers of the given sizes on the current CUDA device; any
     other tensor is refused (its pointer would reach the kernels unchecked)."""
-    out, dev, f32 = [], torch.cuda.current_device(), torch.float32
+    out, f32 = [], torch.float32
+    dev = torch.cuda.current_device() if all(t.is_cuda for t in tensors) else None
     for t, n in zip(tensors, sizes):
         if t.get_device() != dev:
             raise ValueError(f"{who}: tensors must be on the current CUDA device, one is on {t.device}")
