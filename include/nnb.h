@@ -226,6 +226,37 @@ NNB_API nnb_status nnb_layernorm_bwd(void* stream, size_t R, size_t D, const flo
 NNB_API nnb_status nnb_layernorm_bwd_grouped(void* stream, size_t R, size_t D, size_t groups, const float* g,
 		const float* x, const float* gamma, const float* mean, const float* inv_std, float* dx, int dx_first,
 		float* dgamma, size_t dgamma_stride, int dgamma_first, float* dbeta, size_t dbeta_stride, int dbeta_first);
+/* The residual sum after a block joined with the norm before the next one (the reference composes add,
+ * ops.cpp:331, and layernorm, ops.cpp:1003-1078; its RMS norm, gate and scale have no counterpart there):
+ *   p = branch, or norm(branch; post_gamma, post_beta) when post_gamma is not NULL
+ *   h = x + scale * gate * p          gate NULL: 1
+ *   y = norm(h; gamma, beta)
+ * over R rows of D values (D <= 16384). kind NNB_NORM_LAYER: (a - mean) / sqrt(var + eps) * gamma + beta;
+ * NNB_NORM_RMS: a / sqrt(mean a^2 + eps) * gamma, beta and post_beta NULL. gate holds gate_rows rows of D,
+ * each serving R / gate_rows consecutive rows (1: a parameter per channel; ignored when gate is NULL).
+ * stats (R rows of 4 floats, 16-byte aligned; NULL: not kept) is what the backward needs. No other buffer
+ * has an alignment rule; 16 bytes and D % 4 == 0 run fastest. */
+typedef enum nnb_norm_kind { NNB_NORM_LAYER = 0, NNB_NORM_RMS = 1 } nnb_norm_kind;
+NNB_API nnb_status nnb_residual_norm_fwd(void* stream, size_t R, size_t D, size_t gate_rows, int kind, float eps,
+		float scale, const float* x, const float* branch, const float* post_gamma, const float* post_beta,
+		const float* gate, const float* gamma, const float* beta, float* h, float* y, float* stats);
+/* A gradient output: stored (first != 0) or added into p; p NULL skips it. stride: floats between the
+ * groups' gradients of a parameter (0: back to back; unused for dx, dbranch and a gate of several rows). */
+typedef struct nnb_grad_out {
+	float* p;
+	size_t stride;
+	int first;
+} nnb_grad_out;
+/* Gradients of nnb_residual_norm_fwd from dh and dy (either may be NULL: zeros), the forward's h and
+ * stats, and its operands (branch may be NULL without post_gamma and gate). Each nnb_grad_out may be
+ * NULL. dx also receives what reaches h through y. Parameter gradients (a gate of one row included) are
+ * kept per group of R / groups consecutive rows, as nnb_layernorm_bwd_grouped's; a gate of several rows
+ * needs gate_rows % groups == 0. The sums' order depends on D, R / groups and the gate's span only. */
+NNB_API nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups, size_t gate_rows, int kind,
+		float scale, const float* dh, const float* dy, const float* h, const float* branch, const float* post_gamma,
+		const float* post_beta, const float* gate, const float* gamma, const float* stats, const nnb_grad_out* dx,
+		const nnb_grad_out* dbranch, const nnb_grad_out* dpost_gamma, const nnb_grad_out* dpost_beta,
+		const nnb_grad_out* dgate, const nnb_grad_out* dgamma, const nnb_grad_out* dbeta);
 /* Training-mode batchnorm over [N, C, S] (ops.hpp:114; ops.cpp:900-961): per-channel statistics with
  * the reference's fp64 sums of 8-lane partials; fuse_relu folds a ReLU and writes its 1-byte alive
  * mask; mean, var (biased) and inv_std (C each) are written. */

@@ -131,6 +131,9 @@ _SIGS = {
     "nnb_adamw_multi_step": ([_p, _sz, _p, _p, _p, _p, _p, _f, _f, _f, _f, _f, _c.c_longlong], _i),
     "nnb_adamw8_multi_step": ([_p, _sz, _p, _p, _p, _p, _p, _p, _p, _f, _f, _f, _f, _f, _c.c_longlong], _i),
     "nnb_adamw8_moments": ([_p, _sz, _p, _p, _p, _p, _p, _p], _i),
+    "nnb_residual_norm_fwd": ([_p, _sz, _sz, _sz, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p], _i),
+    "nnb_residual_norm_bwd": ([_p, _sz, _sz, _sz, _sz, _i, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                               _p], _i),
     "nnb_manual_seed": ([_c.c_uint64], None),
     "nnb_is_seeded": ([], _i),
     "nnb_seed_epoch": ([], _c.c_uint64),
@@ -149,6 +152,14 @@ _SIGS = {
     "nnb_gather_rows": ([_p, _p, _sz, _sz, _p, _sz, _p], _i),
     "nnb_gather_windows": ([_p, _p, _sz, _p, _sz, _sz, _p, _p], _i),
 }
+
+
+class GradOut(_c.Structure):
+    """nnb_grad_out: a gradient output of nnb_residual_norm_bwd."""
+    _fields_ = [("p", _p), ("stride", _sz), ("first", _i)]
+
+
+NORM_LAYER, NORM_RMS = 0, 1
 
 
 def header_symbols() -> list[str]:

@@ -17,6 +17,8 @@ from typing import Callable, Sequence
 
 import torch
 
+from . import check, lib
+
 
 def empty(shape, dtype=torch.float32, device=None):
     """An uninitialised device buffer (plumbing: no kernel runs)."""
@@ -35,13 +37,15 @@ def _one(device) -> torch.Tensor:
 
 
 class Value:
-    __slots__ = ("data", "grad", "grad_fresh", "requires_grad", "parents", "backward_fn", "name")
+    __slots__ = ("data", "grad", "grad_fresh", "grad_borrowed", "requires_grad", "parents", "backward_fn", "name",
+                 "__weakref__")
 
     def __init__(self, data: torch.Tensor, requires_grad: bool = False, parents: Sequence["Value"] = (),
                  backward_fn: Callable[[torch.Tensor], None] | None = None):
         self.data = data
         self.grad: torch.Tensor | None = None
         self.grad_fresh = False
+        self.grad_borrowed = False           # grad is a caller's seed: read, never written
         self.requires_grad = requires_grad
         self.parents = tuple(parents)
         self.backward_fn = backward_fn
@@ -71,14 +75,21 @@ class Value:
         if self.grad is None:
             self.grad = torch.empty_like(self.data)
             self.grad_fresh = True
+        elif self.grad_borrowed:
+            seed, self.grad = self.grad, torch.empty_like(self.data)
+            if not self.grad_fresh:
+                check(lib().nnb_accumulate(torch.cuda.current_stream().cuda_stream, seed.numel(), seed.data_ptr(),
+                                           self.grad.data_ptr(), 1, 0))
+        self.grad_borrowed = False
         first = 1 if self.grad_fresh else 0
         self.grad_fresh = False
         return self.grad, first
 
     def zero_grad(self) -> None:
         """Marks the gradient as all zeros without writing it (value.cpp:69-76)."""
-        if self.grad is None or self.grad.shape != self.data.shape:
+        if self.grad is None or self.grad.shape != self.data.shape or self.grad_borrowed:
             self.grad = torch.empty_like(self.data)
+            self.grad_borrowed = False
         self.grad_fresh = True
 
     @property
@@ -90,34 +101,48 @@ class Value:
         """Runs the backward rules; the root's gradient is 1, or `seed` (a device tensor with the
         root's element count: an upstream gradient, which lets a non-scalar root be differentiated
         as the reference's tests do with sum(y * g))."""
-        if seed is None and self.data.numel() != 1:
+        backward((self,), (seed,))
+
+
+def backward(roots: Sequence[Value], seeds: Sequence[torch.Tensor | None]) -> None:
+    """Value.backward from several roots at once, each with its upstream gradient (None: 1, for a
+    single-element root): the gradients of the sum over roots of sum(root * seed). A root may depend on
+    another; its own seed and what reaches it through the other are added. The seeds are not written."""
+    if len(roots) != len(seeds) or not roots:
+        raise ValueError("backward(): needs as many seeds as roots, and at least one")
+    if len({id(r) for r in roots}) != len(roots):
+        raise ValueError("backward(): the same root twice")
+    for root, seed in zip(roots, seeds):
+        if seed is None and root.data.numel() != 1:
             raise ValueError("backward() needs a single-element value (AutogradShapeError)")
-        if seed is not None and seed.numel() != self.data.numel():
+        if seed is not None and seed.numel() != root.data.numel():
             raise ValueError("backward(): the seed must have the root's element count")
-        topo: list[Value] = []
-        expanded, done = set(), set()
-        stack = [self]
-        while stack:
-            v = stack[-1]
-            if id(v) in done:
-                stack.pop()
-                continue
-            if id(v) in expanded:
-                stack.pop()
-                done.add(id(v))
-                topo.append(v)
-                continue
-            expanded.add(id(v))
-            for p in v.parents:
-                if id(p) not in expanded:
-                    stack.append(p)
-        for v in topo:
-            if v.backward_fn is not None:
-                if v.grad is None or v.grad.shape != v.data.shape:
-                    v.grad = torch.empty_like(v.data)
-                v.grad_fresh = True
-        self.grad = (_one(self.data.device) if seed is None else seed).view(self.data.shape)
-        self.grad_fresh = False
-        for v in reversed(topo):
-            if v.backward_fn is not None:
-                v.backward_fn(v.grad)
+    topo: list[Value] = []
+    expanded, done = set(), set()
+    stack = list(roots)
+    while stack:
+        v = stack[-1]
+        if id(v) in done:
+            stack.pop()
+            continue
+        if id(v) in expanded:
+            stack.pop()
+            done.add(id(v))
+            topo.append(v)
+            continue
+        expanded.add(id(v))
+        for p in v.parents:
+            if id(p) not in expanded:
+                stack.append(p)
+    for v in topo:
+        if v.backward_fn is not None:
+            if v.grad is None or v.grad.shape != v.data.shape or v.grad_borrowed:
+                v.grad = torch.empty_like(v.data)
+                v.grad_borrowed = False
+            v.grad_fresh = True
+    for root, seed in zip(roots, seeds):
+        root.grad = (_one(root.data.device) if seed is None else seed).view(root.data.shape)
+        root.grad_fresh, root.grad_borrowed = False, True
+    for v in reversed(topo):
+        if v.backward_fn is not None:
+            v.backward_fn(v.grad)

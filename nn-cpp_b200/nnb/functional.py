@@ -11,10 +11,11 @@ import contextlib
 import ctypes
 import math
 import os
+import weakref
 
 import torch
 
-from . import TensorShapeError, check, lib
+from . import NORM_LAYER, NORM_RMS, GradOut, TensorShapeError, check, lib
 from .autograd import Value, empty
 
 
@@ -341,6 +342,93 @@ def layernorm(x: Value, gamma: Value, beta: Value, eps: float) -> Value:
                                               fb))
 
     return Value.node(y, (x, gamma, beta), backward)
+
+
+def _check_buffers(who: str, values, dtype=torch.float32) -> None:
+    """Refuses values that are not contiguous buffers of `dtype` on the current CUDA device (None: skipped)."""
+    tensors = [v.data if isinstance(v, Value) else v for v in values if v is not None]
+    dev = torch.cuda.current_device() if all(t.is_cuda for t in tensors) else None
+    for t in tensors:
+        if t.get_device() != dev:
+            raise ValueError(f"{who}: tensors must be on the current CUDA device, one is on {t.device}")
+        if t.dtype is not dtype or not t.is_contiguous():
+            raise ValueError(f"{who}: tensors must be contiguous {dtype}, one is {t.dtype}")
+
+
+def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = None, eps: float = 1e-5, *,
+                  kind: str = "layer", post_gamma: Value | None = None, post_beta: Value | None = None,
+                  gate: Value | None = None, scale: float = 1.0) -> tuple[Value, Value]:
+    """(h, y) with h = x + scale * gate * p and y = norm(h; gamma, beta): the residual sum after a block
+    and the norm before the next one in one pass. p is the branch, or norm(branch; post_gamma, post_beta)
+    when post_gamma is given.
+
+    kind "layer" normalises by mean and variance and needs the betas, "rms" by the mean square and has
+    none; `eps` serves both norms. The gate's last axis is the width D; its other axes hold n rows in all
+    (none: [D], one row), each for rows / n consecutive rows of x: [D] or [1, D] is a parameter per
+    channel (its gradient kept per parameter group as a norm's is), [N, 1, D] one row per sequence of an
+    x of [N, T, D], x's own shape one per token.
+
+    The backward runs when h's turn comes, with what reached y held until then: the gradient buffer of h
+    itself keeps what its other consumers gave."""
+    if kind not in ("layer", "rms"):
+        raise ValueError('residual_norm: kind must be "layer" or "rms"')
+    layer = kind == "layer"
+    if not x.shape or 0 in x.shape or branch.shape != x.shape:
+        raise TensorShapeError("residual_norm: x and branch need one non-empty shape")
+    D = x.shape[-1]
+    R = x.data.numel() // D
+    if layer != (beta is not None) or (post_beta is not None) != (layer and post_gamma is not None):
+        raise ValueError("residual_norm: a layer norm needs a beta, an rms norm has none")
+    if any(p is not None and p.shape != (D,) for p in (gamma, beta, post_gamma, post_beta)):
+        raise TensorShapeError("residual_norm: norm parameters must be [D]")
+    gate_rows = 0
+    if gate is not None:
+        if not gate.shape or gate.shape[-1] != D or gate.data.numel() == 0 or R % (gate.data.numel() // D):
+            raise TensorShapeError("residual_norm: the gate must be rows of D that divide x's rows")
+        gate_rows = gate.data.numel() // D
+        if gate_rows > 1 and gate_rows % _GROUPS:
+            raise TensorShapeError("residual_norm: the gate's rows do not divide into the parameter groups")
+    if R % _GROUPS:
+        raise TensorShapeError("residual_norm: the rows do not divide into the parameter groups")
+    _check_buffers("residual_norm", (x, branch, gamma, beta, post_gamma, post_beta, gate))
+    k = NORM_LAYER if layer else NORM_RMS
+    opt = lambda v: None if v is None else v.data.data_ptr()
+    h_data, y_data = empty(x.shape), empty(x.shape)
+    stream_parents = tuple(v for v in (x, branch, post_gamma, post_beta, gate) if v is not None)
+    norm_parents = tuple(v for v in (gamma, beta) if v is not None)
+    train = any(_need(v) for v in stream_parents + norm_parents)
+    stats = empty((R, 4)) if train else None
+    check(lib().nnb_residual_norm_fwd(_s(), R, D, gate_rows, k, eps, scale, _p(x.data), _p(branch.data), opt(post_gamma),
+                                      opt(post_beta), opt(gate), _p(gamma.data), opt(beta), _p(h_data), _p(y_data),
+                                      _p(stats)))
+    held = []          # what reached y in the running backward
+
+    def run(dh, dy):
+        def out(v, grouped):
+            if v is None or not _need(v):
+                return None
+            buf, first = v.grad_accum()
+            return ctypes.byref(GradOut(buf.data_ptr(), _gstride(buf, v) if grouped else 0, first))
+        check(lib().nnb_residual_norm_bwd(_s(), R, D, _GROUPS, gate_rows, k, scale, _p(dh), _p(dy), _p(h_data),
+                                          _p(branch.data), opt(post_gamma), opt(post_beta), opt(gate), _p(gamma.data),
+                                          _p(stats), out(x, False), out(branch, False), out(post_gamma, True),
+                                          out(post_beta, True), out(gate, gate_rows == 1),
+                                          *((out(gamma, True), out(beta, True)) if dy is not None else (None, None))))
+
+    def h_backward(g):
+        dy = held.pop() if held else None
+        node = h_ref()
+        run(None if node is not None and node.grad_fresh else g, dy)
+
+    def y_backward(g):
+        if h.requires_grad:
+            held[:] = [g]
+        else:
+            run(None, g)
+
+    h = Value.node(h_data, stream_parents, h_backward)
+    h_ref = weakref.ref(h)
+    return h, Value.node(y_data, (h,) + norm_parents, y_backward)
 
 
 def batchnorm(x: Value, weight: Value, bias: Value, eps: float, fuse_relu: bool = False,
