@@ -228,7 +228,7 @@ def _framework():
 
 
 def _prepare_own(state):
-    nnb = _framework()
+    nnb = state["nnb"] = _framework()
     case, data = state["case"], state["data"]
     leaf = nnb.autograd.Value.leaf
     if case["op"] == "adamw":
@@ -250,7 +250,7 @@ def _prepare_own(state):
 
 
 def _run_own(state):
-    nnb = _framework()
+    nnb = state["nnb"]
     case, data = state["case"], state["data"]
     if case["op"] == "adamw":
         opt = state["opt"]
