@@ -1,5 +1,6 @@
 // nnb_residual_norm.cuh -- what the residual norm's forward and backward share (ops_residual_norm.cu), and
-// the backward kernel, compiled for float4 rows and for single floats in translation units of their own.
+// the backward kernel, whose many instances are compiled in four translation units of their own
+// (ops_residual_norm_{vec,scalar}{,_post}.cu).
 #pragma once
 
 #include <algorithm>
@@ -147,18 +148,24 @@ __device__ __forceinline__ void run_rows(const Grad& p, long long q, long long& 
 	}
 }
 
-// kLayer, kPost, kGate: the form; kMaxT: the CTA's threads, 256, or 512 or 1024 for longer rows. grid = (chunks, groups); dynamic
-// shared memory: the slots' staged rows, then (slots - 1) x D floats, one array of the CTA's sums at a time.
-template <int VEC, int KV, bool kLayer, bool kPost, bool kGate, int kMaxT>
-__global__ void __launch_bounds__(kMaxT, bwd_ctas(kPost || kGate, kMaxT)) residual_norm_bwd_kernel(const Grad p) {
+// T threads per row and KV * VEC columns per thread, known to the compiler (one base address and constant
+// offsets per row); kLayer, kPost, kGate: the form. grid = (chunks, groups); dynamic shared memory: the
+// slots' staged rows, then (slots - 1) x D floats, one array of the CTA's sums at a time.
+template <int VEC, int KV, int T, bool kLayer, bool kPost, bool kGate>
+__global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, T)) residual_norm_bwd_kernel(const Grad p) {
 	extern __shared__ float4 dyn4[];
 	__shared__ float2 buf[2 * 32];
-	const int T = p.T, slot = threadIdx.x / T, slots = blockDim.x / T, t = threadIdx.x - slot * T;
-	const int D = p.D, groups = D / VEC;
-	const float inv_d = 1.0f / (float)D;
-	SlotSum sum(buf, T);
+	constexpr int kSlots = (T > kCta ? T : kCta) / T;
 	constexpr bool kBranch = kPost || kGate;       // the branch is read
 	constexpr int kStaged = staged_arrays(kBranch, VEC * KV);
+	constexpr int kStep = T * VEC;                 // floats between a thread's groups of VEC columns
+	const int slot = threadIdx.x / T, j0 = threadIdx.x % T * VEC;
+	const int D = p.D;
+	const float inv_d = 1.0f / (float)D;
+	SlotSum sum(buf, T);
+	bool in[KV];
+#pragma unroll
+	for (int u = 0; u < KV; ++u) in[u] = j0 + u * kStep < D;
 	Pack<VEC> sg[KV], sb[kLayer ? KV : 1], spg[kPost ? KV : 1], spb[kPost && kLayer ? KV : 1], sgate[kGate ? KV : 1];
 #pragma unroll
 	for (int u = 0; u < KV; ++u) {
@@ -172,24 +179,23 @@ __global__ void __launch_bounds__(kMaxT, bwd_ctas(kPost || kGate, kMaxT)) residu
 	// itself (array a of this slot at stage + a * D), so it needs no barrier, and it issues the next row's
 	// copies as soon as it has taken this row into registers.
 	float* const dyn = reinterpret_cast<float*>(dyn4);
-	float* const stage = dyn + (long long)slot * kStaged * D;
-	auto fetch = [&](long long r) {
-		const long long off = r * D;
+	float* const stage = dyn + slot * kStaged * D + j0;
+	const bool with_dh = p.dh != nullptr, with_dy = p.dy != nullptr;
+	auto fetch = [&](long long off) {
+		auto copy = [&](int array, const float* src) {
 #pragma unroll
-		for (int u = 0; u < KV; ++u) {
-			const int j = (t + u * T) * VEC;
-			if (t + u * T < groups) {
-				if (p.dh) async_copy<VEC>(stage + j, p.dh + off + j);
-				if (p.dy) {
-					async_copy<VEC>(stage + D + j, p.dy + off + j);
-					async_copy<VEC>(stage + 2 * D + j, p.h + off + j);
-				}
-				if constexpr (kStaged == 4) async_copy<VEC>(stage + 3 * D + j, p.branch + off + j);
-			}
+			for (int u = 0; u < KV; ++u)
+				if (in[u]) async_copy<VEC>(stage + array * D + u * kStep, src + off + u * kStep);
+		};
+		if (with_dh) copy(0, p.dh);
+		if (with_dy) {
+			copy(1, p.dy);
+			copy(2, p.h);
 		}
+		if constexpr (kStaged == 4) copy(3, p.branch);
 		cp_async_commit();
 	};
-	const long long q = blockIdx.x * (long long)slots + slot;
+	const long long q = blockIdx.x * (long long)kSlots + slot;
 	long long lo = 0, hi = 0;
 	if (q < p.runs) run_rows(p, q, lo, hi);
 	const long long base = blockIdx.y * p.group_rows;
@@ -199,117 +205,145 @@ __global__ void __launch_bounds__(kMaxT, bwd_ctas(kPost || kGate, kMaxT)) residu
 	if (kGate && lo < hi) {
 		span_index = (base + lo) / p.gate_span;
 		span_left = p.gate_span - (base + lo) % p.gate_span;
-		gate_row = p.gate + span_index * D;
+		gate_row = p.gate + span_index * D + j0;
 	}
-	if (lo < hi) fetch(base + lo);
+	if (lo < hi) fetch((base + lo) * D + j0);
 	for (long long r = base + lo; r < base + hi; ++r) {
-		const long long off = r * D;
+		const long long off = r * D + j0;
 		const float4 st = p.stats[r];
-		cp_async_wait<0>();
-		Pack<VEC> dt[KV], hat[KV], br[KV];
+		Pack<VEC> dt[KV], hat[KV], br[kBranch ? KV : 1];
 		float2 ab = make_float2(0.0f, 0.0f);
+		cp_async_wait<0>();
 #pragma unroll
 		for (int u = 0; u < KV; ++u) {
-			const int j = (t + u * T) * VEC;
-			if (t + u * T < groups) {
-				if (p.dh) dt[u].load_rw(stage + j); else dt[u].zero();
-				if constexpr (kStaged == 4) br[u].load_rw(stage + 3 * D + j);
-				else if constexpr (kBranch) br[u].load(p.branch + off + j);
-				if (p.dy) {
-					Pack<VEC> dy;
-					dy.load_rw(stage + D + j);
-					hat[u].load_rw(stage + 2 * D + j);
-					Pack<VEC> g;
-					g.load(p.gamma + j);
-#pragma unroll
-					for (int i = 0; i < VEC; ++i) {
-						const float x = (hat[u].v[i] - st.x) * st.y, d = dy.v[i] * g.v[i];
-						hat[u].v[i] = x;
-						ab.x += d;
-						ab.y = __fmaf_rn(d, x, ab.y);
-						sg[u].v[i] = __fmaf_rn(dy.v[i], x, sg[u].v[i]);
-						if constexpr (kLayer) sb[u].v[i] += dy.v[i];
-						dt[u].v[i] = __fmaf_rn(st.y, d, dt[u].v[i]);   // dh + inv dhat
-					}
+			dt[u].zero();
+			if (in[u] && with_dh) dt[u].load_rw(stage + u * kStep);
+			if constexpr (kBranch) {
+				br[u].zero();
+				if constexpr (kStaged == 4) {
+					if (in[u]) br[u].load_rw(stage + 3 * D + u * kStep);
+				} else {
+					if (in[u]) br[u].load(p.branch + off + u * kStep);
 				}
 			}
 		}
-		if (r + 1 < base + hi) fetch(r + 1);
-		if (p.dy) {                                    // the same for every thread
-			ab = sum(ab);
-			const float ma = kLayer ? st.y * (ab.x * inv_d) : 0.0f, mb = st.y * (ab.y * inv_d);
+		if (with_dy) {
+#pragma unroll
+			for (int u = 0; u < KV; ++u) {
+				Pack<VEC> dy, g;
+				dy.zero();
+				g.zero();
+				hat[u].zero();
+				if (in[u]) {
+					dy.load_rw(stage + D + u * kStep);
+					hat[u].load_rw(stage + 2 * D + u * kStep);
+					g.load(p.gamma + j0 + u * kStep);
+				}
+#pragma unroll
+				for (int i = 0; i < VEC; ++i) {
+					const float x = (hat[u].v[i] - st.x) * st.y, d = dy.v[i] * g.v[i];
+					hat[u].v[i] = x;
+					ab.x += d;
+					ab.y = __fmaf_rn(d, x, ab.y);
+					sg[u].v[i] = __fmaf_rn(dy.v[i], x, sg[u].v[i]);
+					if constexpr (kLayer) sb[u].v[i] += dy.v[i];
+					dt[u].v[i] = __fmaf_rn(st.y, d, dt[u].v[i]);       // dh + inv dhat
+				}
+			}
+		}
+		if (r + 1 < base + hi) fetch(off + D);
+		if (with_dy) {
+			float ma = 0.0f, mb;
+			if constexpr (kLayer) {
+				ab = sum(ab);
+				ma = st.y * (ab.x * inv_d);
+				mb = st.y * (ab.y * inv_d);
+			} else {
+				mb = st.y * (sum(ab.y) * inv_d);
+			}
 #pragma unroll
 			for (int u = 0; u < KV; ++u)
 #pragma unroll
 				for (int i = 0; i < VEC; ++i) dt[u].v[i] = dt[u].v[i] - ma - hat[u].v[i] * mb;
 		}
+		if (p.dx) {
+#pragma unroll
+			for (int u = 0; u < KV; ++u)
+				if (in[u]) store_grad<VEC>(p.dx + off + u * kStep, dt[u], p.dx_first);
+		}
 		float2 ce = make_float2(0.0f, 0.0f);
 #pragma unroll
 		for (int u = 0; u < KV; ++u) {
-			const int j = (t + u * T) * VEC;
-			if (t + u * T < groups) {
-				if (p.dx) store_grad<VEC>(p.dx + off + j, dt[u], p.dx_first);
-				Pack<VEC> pg, pb;
-				if (kPost) {
-					pg.load(p.post_gamma + j);
-					if constexpr (kLayer) pb.load(p.post_beta + j); else pb.zero();
+			Pack<VEC> pg, pb;
+			if constexpr (kPost) {
+				pg.zero();
+				pb.zero();
+				if (in[u]) pg.load(p.post_gamma + j0 + u * kStep);
+				if constexpr (kLayer && kGate) {
+					if (in[u]) pb.load(p.post_beta + j0 + u * kStep);
 				}
-				if constexpr (kGate) {
-					Pack<VEC> gt;
-					gt.load(gate_row + j);
+			}
+			if constexpr (kGate) {
+				Pack<VEC> gt;
+				gt.zero();
+				if (in[u]) gt.load(gate_row + u * kStep);
 #pragma unroll
-					for (int i = 0; i < VEC; ++i) {
-						const float s = p.scale * dt[u].v[i];
-						const float pv = kPost ? __fmaf_rn((br[u].v[i] - st.z) * st.w, pg.v[i], pb.v[i]) : br[u].v[i];
-						sgate[u].v[i] = __fmaf_rn(s, pv, sgate[u].v[i]);
-						dt[u].v[i] = s * gt.v[i];
-					}
-				} else {
-#pragma unroll
-					for (int i = 0; i < VEC; ++i) dt[u].v[i] *= p.scale;
+				for (int i = 0; i < VEC; ++i) {
+					const float s = p.scale * dt[u].v[i];
+					const float pv = kPost ? __fmaf_rn((br[u].v[i] - st.z) * st.w, pg.v[i], pb.v[i]) : br[u].v[i];
+					sgate[u].v[i] = __fmaf_rn(s, pv, sgate[u].v[i]);
+					dt[u].v[i] = s * gt.v[i];
 				}
-				if constexpr (kPost) {
+			} else {
 #pragma unroll
-					for (int i = 0; i < VEC; ++i) {
-						const float x = (br[u].v[i] - st.z) * st.w, d = dt[u].v[i] * pg.v[i];
-						spg[u].v[i] = __fmaf_rn(dt[u].v[i], x, spg[u].v[i]);
-						if constexpr (kLayer) spb[u].v[i] += dt[u].v[i];
-						br[u].v[i] = x;
-						dt[u].v[i] = d;
-						ce.x += d;
-						ce.y = __fmaf_rn(d, x, ce.y);
-					}
-				} else if (p.dbranch) {
-					store_grad<VEC>(p.dbranch + off + j, dt[u], p.dbranch_first);
+				for (int i = 0; i < VEC; ++i) dt[u].v[i] *= p.scale;
+			}
+			if constexpr (kPost) {
+#pragma unroll
+				for (int i = 0; i < VEC; ++i) {
+					const float x = in[u] ? (br[u].v[i] - st.z) * st.w : 0.0f, d = dt[u].v[i] * pg.v[i];
+					spg[u].v[i] = __fmaf_rn(dt[u].v[i], x, spg[u].v[i]);
+					if constexpr (kLayer) spb[u].v[i] += dt[u].v[i];
+					br[u].v[i] = x;
+					dt[u].v[i] = d;
+					ce.x += d;
+					ce.y = __fmaf_rn(d, x, ce.y);
 				}
 			}
 		}
-		if (kPost) {
-			ce = sum(ce);
-			const float mc = kLayer ? ce.x * inv_d : 0.0f, me = ce.y * inv_d;
-#pragma unroll
-			for (int u = 0; u < KV; ++u) {
-				const int j = (t + u * T) * VEC;
-				if (t + u * T < groups && p.dbranch) {
-#pragma unroll
-					for (int i = 0; i < VEC; ++i) dt[u].v[i] = st.w * (dt[u].v[i] - mc - br[u].v[i] * me);
-					store_grad<VEC>(p.dbranch + off + j, dt[u], p.dbranch_first);
-				}
+		if constexpr (kPost) {
+			float mc = 0.0f, me;
+			if constexpr (kLayer) {
+				ce = sum(ce);
+				mc = ce.x * inv_d;
+				me = ce.y * inv_d;
+			} else {
+				me = sum(ce.y) * inv_d;
 			}
-		}
-		if (kGate && !p.gate_is_param && (--span_left == 0 || r + 1 == base + hi)) {
-			// the last row of a span (or of a piece of one): its sum goes out and starts again
-			const bool piece = p.pieces > 1;
-			float* dst = piece ? p.gate_part + (blockIdx.y * p.runs + q) * D : p.dgate ? p.dgate + span_index * D : nullptr;
-			++span_index;
-			span_left = p.gate_span;
-			gate_row += D;
 #pragma unroll
-			for (int u = 0; u < KV; ++u) {
-				const int j = (t + u * T) * VEC;
-				if (t + u * T < groups) {
-					if (piece) sgate[u].store(dst + j);
-					else if (dst) store_grad<VEC>(dst + j, sgate[u], p.dgate_first);
+			for (int u = 0; u < KV; ++u)
+#pragma unroll
+				for (int i = 0; i < VEC; ++i) dt[u].v[i] = st.w * (dt[u].v[i] - mc - br[u].v[i] * me);
+		}
+		if (p.dbranch) {
+#pragma unroll
+			for (int u = 0; u < KV; ++u)
+				if (in[u]) store_grad<VEC>(p.dbranch + off + u * kStep, dt[u], p.dbranch_first);
+		}
+		if constexpr (kGate) {
+			if (!p.gate_is_param && (--span_left == 0 || r + 1 == base + hi)) {
+				// the last row of a span (or of a piece of one): its sum goes out and starts again
+				const bool piece = p.pieces > 1;
+				float* dst = piece ? p.gate_part + (blockIdx.y * p.runs + q) * D : p.dgate ? p.dgate + span_index * D : nullptr;
+				++span_index;
+				span_left = p.gate_span;
+				gate_row += D;
+#pragma unroll
+				for (int u = 0; u < KV; ++u) {
+					if (in[u] && dst) {
+						if (piece) sgate[u].store(dst + j0 + u * kStep);
+						else store_grad<VEC>(dst + j0 + u * kStep, sgate[u], p.dgate_first);
+					}
 					sgate[u].zero();
 				}
 			}
@@ -322,19 +356,19 @@ __global__ void __launch_bounds__(kMaxT, bwd_ctas(kPost || kGate, kMaxT)) residu
 		if (slot > 0) {
 #pragma unroll
 			for (int u = 0; u < KV; ++u)
-				if (t + u * T < groups) s[u].store(fold + (long long)(slot - 1) * D + (t + u * T) * VEC);
+				if (in[u]) s[u].store(fold + (slot - 1) * D + j0 + u * kStep);
 		}
 		__syncthreads();
 		if (slot == 0) {
-			float* dst = p.part + ((array * (long long)gridDim.y + blockIdx.y) * p.chunks + blockIdx.x) * D;
+			float* dst = p.part + ((array * (long long)gridDim.y + blockIdx.y) * p.chunks + blockIdx.x) * D + j0;
 #pragma unroll
 			for (int u = 0; u < KV; ++u)
-				if (t + u * T < groups) {
-					const int j = (t + u * T) * VEC;
-					for (int k = 0; k + 1 < slots; ++k)
+				if (in[u]) {
 #pragma unroll
-						for (int i = 0; i < VEC; ++i) s[u].v[i] += fold[(long long)k * D + j + i];
-					s[u].store(dst + j);
+					for (int k = 0; k + 1 < kSlots; ++k)
+#pragma unroll
+						for (int i = 0; i < VEC; ++i) s[u].v[i] += fold[k * D + j0 + u * kStep + i];
+					s[u].store(dst + u * kStep);
 				}
 		}
 		__syncthreads();
@@ -348,32 +382,37 @@ __global__ void __launch_bounds__(kMaxT, bwd_ctas(kPost || kGate, kMaxT)) residu
 	}
 }
 
-template <int VEC, int KV, bool kLayer, bool kPost, bool kGate, int kMaxT>
-static nnb_status launch_bwd_as(cudaStream_t s, const Grad& p, long long groups) {
-	const int cta = std::max(p.T, kCta), slots = cta / p.T;
-	const size_t smem = (size_t)slots * staged_arrays(kPost || kGate, VEC * KV) * p.D * sizeof(float);  // holds the fold too
-	auto kernel = residual_norm_bwd_kernel<VEC, KV, kLayer, kPost, kGate, kMaxT>;
-	if (smem > 48 * 1024) NNB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-	kernel<<<dim3((unsigned)p.chunks, (unsigned)groups), cta, smem, s>>>(p);
+template <int VEC, int KV, int T, bool kLayer, bool kPost, bool kGate>
+nnb_status launch_bwd(cudaStream_t s, const Grad& p, long long groups) {
+	constexpr int kThreads = T > kCta ? T : kCta;
+	const size_t smem = (size_t)(kThreads / T) * staged_arrays(kPost || kGate, VEC * KV) * p.D * sizeof(float);  // and the fold
+	auto kernel = residual_norm_bwd_kernel<VEC, KV, T, kLayer, kPost, kGate>;
+	if (smem > 40 * 1024)                          // with the static part: above the default 48 KB
+		NNB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+	kernel<<<dim3((unsigned)p.chunks, (unsigned)groups), kThreads, smem, s>>>(p);
 	return cuda_status(cudaGetLastError(), "residual_norm_bwd launch");
 }
-template <int VEC, int KV, int kMaxT>
-static nnb_status launch_bwd(cudaStream_t s, const Grad& p, long long groups) {
-	const int form = (p.layer ? 4 : 0) + (p.post_gamma ? 2 : 0) + (p.gate ? 1 : 0);
-	switch (form) {
-	case 0: return launch_bwd_as<VEC, KV, false, false, false, kMaxT>(s, p, groups);
-	case 1: return launch_bwd_as<VEC, KV, false, false, true, kMaxT>(s, p, groups);
-	case 2: return launch_bwd_as<VEC, KV, false, true, false, kMaxT>(s, p, groups);
-	case 3: return launch_bwd_as<VEC, KV, false, true, true, kMaxT>(s, p, groups);
-	case 4: return launch_bwd_as<VEC, KV, true, false, false, kMaxT>(s, p, groups);
-	case 5: return launch_bwd_as<VEC, KV, true, false, true, kMaxT>(s, p, groups);
-	case 6: return launch_bwd_as<VEC, KV, true, true, false, kMaxT>(s, p, groups);
-	default: return launch_bwd_as<VEC, KV, true, true, true, kMaxT>(s, p, groups);
+
+// By the threads of a row that the host chose (p.T): eight columns per thread, 16 above 8192.
+template <int VEC, bool kLayer, bool kPost, bool kGate>
+nnb_status dispatch_bwd(cudaStream_t s, const Grad& p, long long groups) {
+	constexpr int kKV = 8 / VEC;
+	if (p.D > 8 * 1024) return launch_bwd<VEC, 2 * kKV, 1024, kLayer, kPost, kGate>(s, p, groups);
+	switch (p.T) {
+	case 32: return launch_bwd<VEC, kKV, 32, kLayer, kPost, kGate>(s, p, groups);
+	case 64: return launch_bwd<VEC, kKV, 64, kLayer, kPost, kGate>(s, p, groups);
+	case 128: return launch_bwd<VEC, kKV, 128, kLayer, kPost, kGate>(s, p, groups);
+	case 256: return launch_bwd<VEC, kKV, 256, kLayer, kPost, kGate>(s, p, groups);
+	case 512: return launch_bwd<VEC, kKV, 512, kLayer, kPost, kGate>(s, p, groups);
+	default: return launch_bwd<VEC, kKV, 1024, kLayer, kPost, kGate>(s, p, groups);
 	}
 }
 
-nnb_status residual_norm_bwd_vec(cudaStream_t s, const Grad& p, long long groups);
-nnb_status residual_norm_bwd_scalar(cudaStream_t s, const Grad& p, long long groups);
+// The backward of rows that move as float4 (vec) or as single floats, with and without post's norm.
+nnb_status bwd_vec(cudaStream_t s, const Grad& p, long long groups);
+nnb_status bwd_vec_post(cudaStream_t s, const Grad& p, long long groups);
+nnb_status bwd_scalar(cudaStream_t s, const Grad& p, long long groups);
+nnb_status bwd_scalar_post(cudaStream_t s, const Grad& p, long long groups);
 
 }  // namespace resnorm
 }  // namespace nnb

@@ -329,23 +329,22 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 	const bool vec = D % 4 == 0 && aligned16({dh, dy, h, branch, post_gamma, post_beta, gate, gamma, gx.p, gb.p, p.dgate});
 	p.T = threads_per_row(p.D, 8);
 
-	// Runs. A whole wave of the GPU's threads over a group's rows, and at least one row each; with a gate
-	// per span a run is whole spans or a piece of one, so that a span's sum is in one or in few runs.
-	const int slots = std::max(p.T, kCta) / p.T;
+	// Runs: as many as one wave of the GPU has slots, over a group's rows. With a gate per span a run is
+	// whole spans or a piece of one, so that a span's sum is in one or in few runs.
+	const int max_t = std::max(p.T, kCta), slots = max_t / p.T;
 	p.group_rows = (long long)(R / groups);
 	p.span = gate && !gate_param ? p.gate_span : p.group_rows;
-	const int max_t = std::max(p.T, kCta);
-	const long long wave = 148LL * max_t * bwd_ctas(needs_branch, max_t), want = std::max<long long>(1, (p.group_rows * p.T + wave - 1) / wave);
-	if (p.span <= want) {
-		p.spans_per_run = want / p.span;
+	const long long wave = 148LL * slots * bwd_ctas(needs_branch, max_t), spans = p.group_rows / p.span;
+	if (spans >= wave) {
+		p.spans_per_run = (spans + wave - 1) / wave;
 		p.run_rows = 0;
 		p.pieces = 1;
-		p.runs = (p.group_rows / p.span + p.spans_per_run - 1) / p.spans_per_run;
+		p.runs = (spans + p.spans_per_run - 1) / p.spans_per_run;
 	} else {
 		p.spans_per_run = 0;
-		p.run_rows = want;
-		p.pieces = (p.span + want - 1) / want;
-		p.runs = p.group_rows / p.span * p.pieces;
+		p.run_rows = (p.span + std::min(p.span, wave / spans) - 1) / std::min(p.span, wave / spans);
+		p.pieces = (p.span + p.run_rows - 1) / p.run_rows;
+		p.runs = spans * p.pieces;
 	}
 	const long long chunks = (p.runs + slots - 1) / slots;
 	if (chunks > INT32_MAX) return fail(NNB_ERR_UNSUPPORTED, "%s: too many rows", who);
@@ -360,7 +359,8 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 	nnb_status st;
 	{
 		TraceScope ts(s, kTraceRowwise);
-		st = vec ? residual_norm_bwd_vec(s, p, (long long)groups) : residual_norm_bwd_scalar(s, p, (long long)groups);
+		st = vec ? (post_gamma ? bwd_vec_post : bwd_vec)(s, p, (long long)groups)
+			: (post_gamma ? bwd_scalar_post : bwd_scalar)(s, p, (long long)groups);
 	}
 	Outs o;
 	const nnb_grad_out outs[kArrays] = {pick(dgamma), pick(dbeta), pick(dpost_gamma), pick(dpost_beta), gate_param ? gg : none};

@@ -1,15 +1,14 @@
-// ops_residual_norm_scalar.cu -- the residual norm's backward for rows of any length and alignment, as the
-// float4 form with single floats.
+// ops_residual_norm_scalar.cu -- instances of the residual norm's backward: rows of any length and alignment, moved as single floats,
+// without a norm after the block.
 #include "nnb_residual_norm.cuh"
 
 namespace nnb {
 namespace resnorm {
 
-nnb_status residual_norm_bwd_scalar(cudaStream_t s, const Grad& p, long long groups) {
-	if (p.D > 8 * 1024) return launch_bwd<1, 16, 1024>(s, p, groups);
-	if (p.T > 512) return launch_bwd<1, 8, 1024>(s, p, groups);
-	if (p.T > kCta) return launch_bwd<1, 8, 512>(s, p, groups);
-	return launch_bwd<1, 8, kCta>(s, p, groups);
+nnb_status bwd_scalar(cudaStream_t s, const Grad& p, long long groups) {
+	if (p.layer)
+		return p.gate ? dispatch_bwd<1, true, false, true>(s, p, groups) : dispatch_bwd<1, true, false, false>(s, p, groups);
+	return p.gate ? dispatch_bwd<1, false, false, true>(s, p, groups) : dispatch_bwd<1, false, false, false>(s, p, groups);
 }
 
 }  // namespace resnorm

@@ -141,7 +141,7 @@ def _run(ops, dh, dy, kind, scale, only=None, base=None):
 
 FORMS = list(itertools.product(("layer", "rms"), (False, True), ("none", "channel", "sequence", "token")))
 SHAPES = [(1, 1, 1), (1, 64, 1), (6, 3, 2), (40, 33, 8), (33, 64, 33), (300, 100, 3), (96, 512, 32), (50, 1001, 25),
-          (12, 1024, 4), (21, 2048, 7), (10, 2500, 5), (9, 4100, 3), (7, 5001, 7), (6, 8192, 2), (5, 16383, 5),
+          (12, 1024, 4), (21, 2048, 7), (10, 2500, 5), (8, 4096, 4), (9, 4100, 3), (7, 5001, 7), (6, 8192, 2), (5, 16383, 5),
           (4, 16384, 2)]
 
 
