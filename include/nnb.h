@@ -412,6 +412,24 @@ NNB_API nnb_status nnb_sequence_ce_fwd(void* stream, size_t P, size_t V, const f
 NNB_API nnb_status nnb_sequence_ce_bwd(void* stream, size_t P, size_t V, const float* softmax,
 		const int64_t* targets, int64_t ignore_index, float label_smoothing, const float* grad_loss,
 		const float* norm, float* dlogits, int first);
+/* sequence_cross_entropy (ops.cpp:1908-1979) of linear(x, w, bias) (ops.cpp:714-745) without keeping the
+ * logits: x [P, D], w [V, D], bias [V] or NULL, targets (device int64) [P]. loss and norm are
+ * nnb_sequence_ce_fwd's (NaN loss when no row counts; an out-of-range target makes the loss NaN and sets
+ * the device error word); row_loss [P] (nullable) receives each row's loss, 0 where the target is
+ * ignore_index. The rows are processed in pieces whose logits (at most 256 MiB, or 128 rows) and their
+ * packed copies live in scratch memory, in the process default math mode.
+ * dx [P, D], dw [V, D], db [V] (each nullable; all NULL: no gradients are computed) receive the gradients
+ * of the SUM of the row losses: the backward of the mean multiplies them by grad_loss * norm
+ * (nnb_scaled_accumulate). dw and db are kept per group of P / groups consecutive rows, dw_stride and
+ * db_stride apart (0: back to back), as nnb_linear_bwd_grouped's; a group's sums depend on its own rows
+ * only. A row whose logits have no finite maximum (all -inf, or NaN) has loss and gradients NaN. */
+NNB_API nnb_status nnb_linear_ce_fwd(void* stream, size_t P, size_t D, size_t V, size_t groups, const float* x,
+		const float* w, const float* bias, const int64_t* targets, int64_t ignore_index, float label_smoothing,
+		float* row_loss, float* loss, float* norm, float* dx, float* dw, size_t dw_stride, float* db, size_t db_stride);
+/* dst_z (+)= src_z * (a * b) for `groups` runs of n values, src back to back, dst dst_stride apart (0: back
+ * to back); a and b are device scalars. */
+NNB_API nnb_status nnb_scaled_accumulate(void* stream, size_t groups, size_t n, const float* src, const float* a,
+		const float* b, float* dst, size_t dst_stride, int first);
 /* embedding (ops.cpp:1991-2015): out[i] = weight[ids[i]]; the backward adds g rows into dweight in
  * token order per row (deterministic, no float atomics), starting from 0 when first != 0 and from
  * dweight's contents otherwise; V <= 40000 for the backward. */

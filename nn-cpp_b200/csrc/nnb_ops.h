@@ -7,6 +7,8 @@
 
 namespace nnb {
 
+constexpr int kDevBadIndex = 16;   // device error word: a target or token id outside its range
+
 // out[j] (+)= sum over rows of g[r][j] in the fixed chunked order of ops_linear.cu.
 nnb_status colsum(cudaStream_t s, const float* g, long long rows, long long cols, float* out, int first);
 // dX (+)= G W and dW_z (+)= G_z^T X_z (per group of rows) of a linear backward; either may be null.

@@ -19,7 +19,6 @@ namespace nnb {
 
 namespace {
 
-constexpr int kDevBadIndex = 16;   // device error word: a target or token id outside its range
 
 #define GRID_STRIDE(i, n) \
 	for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < (n); i += (long long)gridDim.x * blockDim.x)

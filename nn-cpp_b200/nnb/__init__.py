@@ -134,6 +134,8 @@ _SIGS = {
     "nnb_residual_norm_fwd": ([_p, _sz, _sz, _sz, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p], _i),
     "nnb_residual_norm_bwd": ([_p, _sz, _sz, _sz, _sz, _i, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
                                _p], _i),
+    "nnb_linear_ce_fwd": ([_p, _sz, _sz, _sz, _sz, _p, _p, _p, _p, _c.c_int64, _f, _p, _p, _p, _p, _p, _sz, _p, _sz], _i),
+    "nnb_scaled_accumulate": ([_p, _sz, _sz, _p, _p, _p, _p, _sz, _i], _i),
     "nnb_manual_seed": ([_c.c_uint64], None),
     "nnb_is_seeded": ([], _i),
     "nnb_seed_epoch": ([], _c.c_uint64),

@@ -813,3 +813,61 @@ def sequence_cross_entropy(logits: Value, targets: torch.Tensor, ignore_index: i
                                         _p(g), _p(norm if grad_norm is None else grad_norm), _p(dl), f))
 
     return Value.node(loss, (logits,), backward)
+
+
+def _linear_ce_args(who: str, x, weight, bias, targets):
+    """Shapes and buffers of a vocabulary projection's loss: (P, D, V)."""
+    xs, ws = x.shape, weight.shape
+    if len(xs) < 2 or len(ws) != 2 or xs[-1] != ws[1] or 0 in xs or 0 in ws or (bias is not None and bias.shape != ws[:1]):
+        raise TensorShapeError(f"{who}: shapes do not agree")
+    if tuple(targets.shape) != xs[:-1]:
+        raise TensorShapeError(f"{who}: targets must have x's shape without its last axis")
+    _check_buffers(who, (x, weight, bias))
+    _check_buffers(who, (targets,), torch.int64)
+    return x.data.numel() // xs[-1], xs[-1], ws[0]
+
+
+def linear_cross_entropy(x: Value, weight: Value, bias: Value | None, targets: torch.Tensor, ignore_index: int = -100,
+                         label_smoothing: float = 0.0, grad_norm: torch.Tensor | None = None) -> Value:
+    """sequence_cross_entropy(linear(x, weight, bias), targets) without keeping the logits: x [..., D],
+    weight [V, D], bias [V] or None, targets (int64, on the device) of x's leading shape. The mean loss over
+    the targets that are not ignore_index, label smoothing and grad_norm as sequence_cross_entropy's.
+
+    The rows go through in pieces; where a gradient is needed it is computed with the loss, from the same
+    logits, and the backward only scales it (nnb_linear_ce_fwd, include/nnb.h). For inputs that need
+    none, see linear_token_losses."""
+    P, D, V = _linear_ce_args("linear_cross_entropy", x, weight, bias, targets)
+    parents = (x, weight) if bias is None else (x, weight, bias)
+    params = any(_need(v) for v in parents[1:])
+    groups = _GROUPS if params else 1
+    if P % groups:
+        raise TensorShapeError("linear_cross_entropy: the rows do not divide into the parameter groups")
+    loss, norm = empty((1,)), empty((1,))
+    dx = empty((P, D)) if _need(x) else None
+    dw = empty((groups, V, D)) if _need(weight) else None
+    db = empty((groups, V)) if bias is not None and _need(bias) else None
+    check(lib().nnb_linear_ce_fwd(_s(), P, D, V, groups, _p(x.data), _p(weight.data), None if bias is None else _p(bias.data),
+                                  _p(targets), ignore_index, label_smoothing, None, _p(loss), _p(norm), _p(dx), _p(dw), 0,
+                                  _p(db), 0))
+
+    def backward(g):
+        k = norm if grad_norm is None else grad_norm
+        for v, d in ((x, dx), (weight, dw), (bias, db)):
+            if d is not None:
+                buf, f = v.grad_accum()
+                n = v.data.numel()
+                check(lib().nnb_scaled_accumulate(_s(), d.numel() // n, n, _p(d), _p(g), _p(k), _p(buf), _gstride(buf, v), f))
+
+    return Value.node(loss, parents, backward)
+
+
+def linear_token_losses(x: Value, weight: Value, bias: Value | None, targets: torch.Tensor, ignore_index: int = -100,
+                        label_smoothing: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(each target's loss, their mean) of linear_cross_entropy, for evaluation: plain tensors, of the
+    targets' shape (0 where the target is ignore_index) and [1], with no gradients and nothing kept."""
+    P, D, V = _linear_ce_args("linear_token_losses", x, weight, bias, targets)
+    losses, loss, norm = empty(tuple(targets.shape)), empty((1,)), empty((1,))
+    check(lib().nnb_linear_ce_fwd(_s(), P, D, V, 1, _p(x.data), _p(weight.data), None if bias is None else _p(bias.data),
+                                  _p(targets), ignore_index, label_smoothing, _p(losses), _p(loss), _p(norm), None, None, 0,
+                                  None, 0))
+    return losses, loss

@@ -1,0 +1,53 @@
+"""Refusals of the vocabulary projection's loss (host checks only, no GPU needed)."""
+import pytest
+import torch
+
+import nnb
+from nnb import TensorShapeError
+from nnb import functional as F
+from nnb.autograd import Value
+
+P = 16          # an address that is never dereferenced: the checks come first
+
+
+def _fwd(rows=4, D=8, V=8, groups=1, x=P, w=P, bias=P, targets=P, ls=0.0, loss=P, norm=P, dx=P, dw=P, dws=0, db=P, dbs=0):
+    return nnb.lib().nnb_linear_ce_fwd(None, rows, D, V, groups, x, w, bias, targets, -100, ls, None, loss, norm, dx, dw, dws,
+                                       db, dbs)
+
+
+def test_refusals():
+    INV, SHAPE, UNSUP = nnb.NNB_ERR_INVALID, nnb.NNB_ERR_SHAPE, nnb.NNB_ERR_UNSUPPORTED
+    for k in ("rows", "D", "V"):
+        assert _fwd(**{k: 0}) == SHAPE, k
+    assert _fwd(groups=3) == SHAPE and _fwd(groups=0) == SHAPE
+    for ls in (-0.1, 1.0, float("nan")):
+        assert _fwd(ls=ls) == INV and "label_smoothing" in nnb.last_error()
+    for k in ("x", "w", "targets", "loss", "norm"):
+        assert _fwd(**{k: None}) == INV, k
+    assert _fwd(bias=None) == INV and "bias" in nnb.last_error()
+    assert _fwd(groups=2, dws=63) == INV and _fwd(groups=2, dbs=7) == INV and "overlap" in nnb.last_error()
+    assert _fwd(rows=2 ** 31) == UNSUP and _fwd(V=2 ** 31) == UNSUP and _fwd(D=2 ** 31) == UNSUP
+
+
+def test_scaled_accumulate_refusals():
+    f = nnb.lib().nnb_scaled_accumulate
+    assert f(None, 0, 4, None, None, None, None, 0, 1) == nnb.NNB_OK
+    assert f(None, 2, 0, None, None, None, None, 0, 1) == nnb.NNB_OK
+    for i in range(4):
+        assert f(None, 1, 4, *[None if j == i else P for j in range(4)], 0, 1) == nnb.NNB_ERR_INVALID
+    assert f(None, 2, 4, P, P, P, P, 3, 1) == nnb.NNB_ERR_INVALID
+    assert f(None, 70000, 4, P, P, P, P, 0, 1) == nnb.NNB_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("op", [F.linear_cross_entropy, F.linear_token_losses])
+def test_function_refusals(op):
+    v = lambda *s: Value(torch.zeros(s))      # noqa: E731
+    t = torch.zeros(2, 3, dtype=torch.int64)
+    good = (v(2, 3, 8), v(5, 8), v(5))
+    for x, w, b, tt in ((v(8), *good[1:], t), (good[0], v(5, 7), good[2], t), (good[0], v(8), good[2], t),
+                        (*good[:2], v(6), t), (*good, t[:1]), (*good, t.view(-1)), (v(0, 3, 8), *good[1:], t[:0]),
+                        (v(2, 3, 0), v(5, 0), good[2], t)):
+        with pytest.raises(TensorShapeError):
+            op(x, w, b, tt)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        op(*good, t)
