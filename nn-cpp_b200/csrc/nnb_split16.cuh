@@ -1,0 +1,110 @@
+// nnb_split16.cuh -- products of fp32 matrices on the 16-bit tensor-core path: every operand is scaled by a
+// power of two and written as two fp16 parts, x s ~= hi + lo, and C = Ahi Bhi + Ahi Blo + Alo Bhi in fp32.
+//
+// fp16 has the 11 significant bits of TF32 and twice its MMA rate, so the split carries the 22 bits of
+// 3xTF32 at half the time; what fp16 lacks is range. With s = 2^(14 - floor(log2 max|x|)) the largest
+// magnitude lands in [2^14, 2^15): elements down to 2^-17 of it keep their 22 bits (the low part's last
+// bit is 2^-24), smaller ones an absolute error of 2^-40 of the largest. That is fp32 grade next to the
+// sums such elements enter; it is not for operands whose tiny elements count alone, and the general GEMM
+// (gemm.cu) stays with TF32. With one part (TF32 mode) the 11 bits are TF32's own.
+//
+// Precision of the sums: the tensor core adds with truncation, a bias that grows with the number of
+// additions (measured on the TF32 path: 1e-5 of a sum of 1024 terms). So an accumulator holds kChunkKb
+// k-blocks (128 terms, 24 additions) and is then added, rounded to nearest, into registers.
+//
+// Packed layout: blocks of 128 rows x 64 columns, hi part then lo part (16 KB each, rows of 128 bytes),
+// block (rb, c) at index rb * kw + c. The same pack is read K-major (its rows are C's rows or columns) or
+// MN-major (its rows are the depth).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "nnb_internal.h"
+#include "nnb_ptx.cuh"
+
+namespace nnb {
+namespace split16 {
+
+constexpr int kRows = 128, kCols = 64;           // of a packed block
+constexpr int kPartBytes = kRows * kCols * 2;
+constexpr int kBlockBytes = 2 * kPartBytes;      // also 128 x 64 floats
+constexpr int kBM = 128, kBN = 256;              // tile of C
+constexpr int kBK = 32;                          // depth per pipeline stage: rows of 64 bytes
+constexpr int kChunkKb = 4;                      // k-blocks per accumulator
+constexpr int kEpiWarps = 8;                     // two per TMEM lane quarter, 128 columns each
+constexpr int kThreads = 128 + 32 * kEpiWarps;   // producer, MMA issuer, two idle warps, epilogue
+
+// A packed matrix of `rows` x `cols`, rows padded to whole blocks of 128 (256 for a K-major B), columns to 64.
+struct Pack {
+	const void* buf = nullptr;
+	long long rows = 0, cols = 0;
+	long long row_blocks() const { return (rows + kRows - 1) / kRows; }
+	long long kw() const { return (cols + kCols - 1) / kCols; }
+};
+// Bytes of a pack whose rows are padded to an even number of blocks.
+inline size_t pack_bytes(long long rows, long long cols) {
+	return (size_t)((rows + 2 * kRows - 1) / (2 * kRows) * 2) * ((cols + kCols - 1) / kCols) * kBlockBytes;
+}
+
+// A matrix's range on the device: the bit pattern of its largest finite magnitude, and whether it holds an
+// infinity or NaN.
+struct Range {
+	unsigned top, bad;
+};
+// 2^k, -126 <= k <= 127.
+__device__ __forceinline__ float exp2_int(int k) { return __int_as_float((k + 127) << 23); }
+// s = 2^shift(range): the scale that puts the largest magnitude into [2^14, 2^15).
+__device__ __forceinline__ int range_shift(const Range* r) {
+	const unsigned top = r->top;
+	if (top == 0) return 0;
+	const int k = 14 - ((int)(top >> 23) - 127);
+	return k > 126 ? 126 : k;
+}
+
+enum Epilogue : int {
+	kStore = 0,     // C (+)= alpha acc, row-major
+	kStats = 1,     // softmax statistics of acc + bias per row and 128 columns
+	kLogits = 2     // the same, and acc + bias into 128 x 64 float blocks
+};
+
+struct Product {
+	int M = 0, N = 0;
+	int kb = 0;                       // k-blocks of 32
+	int tiles_m = 0, tiles_n = 0;
+	int splits = 1, split_kb = 0;     // depth splits (kStore: split i writes slab i of C), k-blocks each
+	int a_kw = 0, b_kw = 0;           // packed columns of the operands
+	const Range *ra = nullptr, *rb = nullptr;   // ranges that scale acc back (null: none); see `shift`
+	int shift = 0;                    // acc is also multiplied by 2^-shift
+	// kStore
+	float* C = nullptr;
+	long long ldc = 0, slab = 0;
+	int accumulate = 0;
+	// kStats, kLogits
+	const float* bias = nullptr;
+	const int64_t* targets = nullptr; // per row of C
+	float2* part = nullptr;           // [2 tiles_n][rows of whole tiles]: max, sum of exp(l - max)
+	float* part_sum = nullptr;        // the same: sum of l (null: not wanted)
+	float* target_logit = nullptr;    // per row of C
+	float* blocks = nullptr;          // kLogits: [tiles_m][blocks_kw][128][64]
+	int blocks_kw = 0;
+	int* err = nullptr;
+};
+
+// Range of x[rows x cols] (leading dimension cols) into *out (zeroed here).
+nnb_status find_range(cudaStream_t s, const float* x, long long n, Range* out);
+// Packs x [rows x cols] (row-major, dense) into buf, rows padded with zeros to `row_blocks` blocks; values that
+// are not finite become zero and set row_bad[row] (nullable, zeroed by the caller).
+nnb_status pack(cudaStream_t s, const float* x, long long rows, long long cols, long long row_blocks, int parts,
+		const Range* range, void* buf, int* row_bad);
+
+// C = A B^T with A = a (K-major: rows of a) or a^T (mn_a: columns of a), B likewise; p's sizes, operands'
+// widths and tile counts are filled in here. parts: 2 or 1.
+nnb_status run(cudaStream_t s, Product p, int epilogue, int parts, const Pack& a, bool mn_a, const Pack& b, bool mn_b,
+		long long M, long long N, long long K);
+// Depth splits that fill the GPU for an M x N product of depth K; depends on the sizes only.
+int choose_splits(long long M, long long N, long long K);
+// c (+)= sum over `splits` slabs of n floats, in order.
+nnb_status sum_slabs(cudaStream_t s, const float* slabs, int splits, long long n, float* c, int accumulate);
+
+}  // namespace split16
+}  // namespace nnb

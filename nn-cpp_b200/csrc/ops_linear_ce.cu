@@ -5,98 +5,176 @@
 //   G = softmax(l) - s / V - (1 - s) [v = t]   (rows that count; zero elsewhere)
 //   dX = G W,  dW = G^T X,  db = column sums of G        -- of the SUM of the losses
 //
-// The rows go in pieces: one piece's logits are in a scratch buffer at a time. When gradients are wanted
-// they are computed right there, from the same logits, so that the three products cost 6 P V D operations;
-// recomputing the logits in the backward pass would cost 8. The backward pass scales them by the upstream
-// gradient over the number of rows that count, which is known only at the end.
+// The rows go in pieces. A piece's logits come out of the tensor core (split16.cu) with their softmax
+// statistics per row and 128 columns; where no gradient is wanted that is all, and the logits are never
+// written. Else they go into 128 x 64 blocks, which the next kernel turns into G in place: two fp16 parts
+// take the 4 bytes that an fp32 logit took. G is read twice, K-major for dX and MN-major for dW, W and X
+// likewise from one pack each. The three products cost 6 P V D operations; recomputing the logits in the
+// backward pass would cost 8. The backward pass only scales the gradients by the upstream gradient over
+// the number of rows that count, which is known at the end.
+//
+// Ranges (split16): X and W are scaled by their largest magnitude, G by 2^15 (|G| <= 1): an entry of G below
+// 2^-17 loses relative precision, down to an absolute 2^-40, next to the -1 of its row's target.
 #include <algorithm>
 #include <cmath>
 
-#include "nnb_gemm.h"
 #include "nnb_internal.h"
 #include "nnb_ops.h"
+#include "nnb_split16.cuh"
 #include "nnb_trace.h"
 
 namespace nnb {
 
 namespace {
 
-constexpr int kRowThreads = 256;
-constexpr size_t kPieceBytes = size_t(256) << 20;   // logits of one piece
+using split16::kBlockBytes;
+using split16::kCols;
+using split16::kRows;
 
-__device__ __forceinline__ float2 combine(float2 a, float2 b) {
-	// (max, sum of exp(l - max)) of two parts; an empty part is (-inf, 0)
-	const float m = fmaxf(a.x, b.x);
-	if (m == -INFINITY) return make_float2(m, a.y + b.y);
-	return make_float2(m, a.y * expf(a.x - m) + b.y * expf(b.x - m));
+constexpr size_t kPieceBytes = size_t(512) << 20;   // G (and the logits before it) of one piece
+constexpr size_t kPartBytes = size_t(256) << 20;    // softmax statistics of one piece
+constexpr int kGShift = 15;                         // G is packed times 2^15
+constexpr float kLog2e = 1.44269504088896341f;
+
+// What the gradient needs of a row.
+struct RowInfo {
+	float top, inv;      // its largest logit and 1 / sum of exp(l - top); NaN inv: the row is NaN
+	int target;          // -1: the row does not count (ignored, out of range or padding)
+	int unused;
+};
+
+// A row's statistics from its parts (32 rows per CTA, eight threads to a row), its loss and RowInfo.
+__global__ void __launch_bounds__(256) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ part_sum,
+		const float* __restrict__ target_logit, int parts, int rows, int rows_pad, int V, const int64_t* __restrict__ targets,
+		int64_t ignore_index, float ls, const int* __restrict__ x_bad, const split16::Range* __restrict__ w_range,
+		float* __restrict__ row_loss, int* __restrict__ valid, RowInfo* __restrict__ info, int* err) {
+	__shared__ float2 ms[8][32];
+	__shared__ float tot[8][32];
+	const int x = threadIdx.x & 31, y = threadIdx.x >> 5, r = blockIdx.x * 32 + x;
+	float top = -INFINITY, sum = 0.0f, total = 0.0f;
+	// (an empty part is (-inf, 0); a NaN or infinite logit leaves a NaN sum, and so does +inf as a maximum)
+	auto join = [&](float2 b) {
+		const float m = fmaxf(top, b.x);
+		if (m == -INFINITY) {
+			sum += b.y;
+		} else {
+			sum = sum * exp2_hw((top - m) * kLog2e) + b.y * exp2_hw((b.x - m) * kLog2e);
+		}
+		top = m;
+	};
+	if (r < rows)
+#pragma unroll 4
+		for (int k = y; k < parts; k += 8) {
+			join(part[(long long)k * rows_pad + r]);
+			if (part_sum) total += part_sum[(long long)k * rows_pad + r];
+		}
+	ms[y][x] = make_float2(top, sum);
+	tot[y][x] = total;
+	__syncthreads();
+	if (y != 0 || r >= rows_pad) return;
+	RowInfo o = {0.0f, 0.0f, -1, 0};
+	if (r < rows) {
+#pragma unroll
+		for (int k = 1; k < 8; ++k) {
+			join(ms[k][x]);
+			total += tot[k][x];
+		}
+		const int64_t t = targets[r];
+		if (t == ignore_index || t < 0 || t >= V) {
+			row_loss[r] = t == ignore_index ? 0.0f : __int_as_float(0x7fc00000);
+			valid[r] = 0;
+			if (t != ignore_index) atomicCAS(err, 0, kDevBadIndex);
+		} else {
+			// no finite maximum, or a value of x or w that is not finite (packed as zero): NaN
+			if (!(top > -INFINITY && top < INFINITY) || x_bad[r] || w_range->bad) sum = __int_as_float(0x7fc00000);
+			const float lse = logf(sum), nll = lse - (target_logit[r] - top);
+			row_loss[r] = ls == 0.0f ? nll : (1.0f - ls) * nll + ls * (lse - (total / (float)V - top));
+			valid[r] = 1;
+			o.top = top;
+			o.inv = 1.0f / sum;
+			o.target = (int)t;
+		}
+	}
+	if (info) info[r] = o;
 }
 
-// One CTA per row of logits: the row's loss and, when grad, its row of G in place of the logits.
-__global__ void __launch_bounds__(kRowThreads) ce_row_kernel(float* __restrict__ logits, int V,
-		const int64_t* __restrict__ targets, int64_t ignore_index, float ls, int grad, float* __restrict__ row_loss,
-		int* __restrict__ valid, int* err) {
-	__shared__ float2 part[kRowThreads / 32];
-	__shared__ float part_s[kRowThreads / 32];
-	const long long r = blockIdx.x;
-	float* row = logits + r * V;
-	const int64_t t = targets[r];
-	const bool ignored = t == ignore_index;
-	if (ignored || t < 0 || t >= V) {
-		if (grad)
-			for (int c = threadIdx.x; c < V; c += kRowThreads) row[c] = 0.0f;
-		if (threadIdx.x == 0) {
-			row_loss[r] = ignored ? 0.0f : __int_as_float(0x7fc00000);
-			valid[r] = 0;
-			if (!ignored) atomicCAS(err, 0, kDevBadIndex);
-		}
-		return;
-	}
-	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-	float2 ms = make_float2(-INFINITY, 0.0f);
-	float total = 0.0f;
-	for (int c = threadIdx.x; c < V; c += kRowThreads) {
-		const float l = row[c];
-		total += l;
-		if (l > ms.x) {
-			ms.y = ms.y * expf(ms.x - l) + 1.0f;
-			ms.x = l;
-		} else {
-			ms.y += l == -INFINITY && ms.x == -INFINITY ? 0.0f : expf(l - ms.x);
-		}
-	}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+	const __half2 h = __floats2half2_rn(a, b);
+	return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One block of 128 rows x 64 columns per CTA, in place: logits in, G out as fp16 parts; its column sums.
+// A thread holds four columns of eight rows. HBM bound: 4 bytes in and 4 out per logit.
+__global__ void __launch_bounds__(256) ce_grad_kernel(float* __restrict__ blocks, int kw, int V, int rows_pad,
+		const RowInfo* __restrict__ info, float ls, int two_parts, float* __restrict__ col_part) {
+	__shared__ float4 sums[8][16];
+	const int c64 = blockIdx.x, rb = blockIdx.y, tid = threadIdx.x, q = tid & 15, r0 = tid >> 4;
+	float* block = blocks + ((long long)rb * kw + c64) * (kRows * kCols);
+	const int col = c64 * kCols + q * 4;
+	const float spread = ls / (float)V, scale = exp2f((float)kGShift);
+	float4 l[8];
+	RowInfo in[8];
 #pragma unroll
-	for (int o = 16; o > 0; o >>= 1) {
-		ms = combine(ms, make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o)));
-		total += __shfl_xor_sync(0xffffffffu, total, o);
+	for (int i = 0; i < 8; ++i) {
+		l[i] = reinterpret_cast<const float4*>(block)[(r0 + 16 * i) * (kCols / 4) + q];
+		in[i] = info[rb * kRows + r0 + 16 * i];
 	}
-	if (lane == 0) {
-		part[warp] = ms;
-		part_s[warp] = total;
+	float4 cs = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+	for (int i = 0; i < 8; ++i) {
+		float g[4] = {l[i].x, l[i].y, l[i].z, l[i].w};
+#pragma unroll
+		for (int k = 0; k < 4; ++k) {
+			float v = exp2_hw((g[k] - in[i].top) * kLog2e) * in[i].inv - spread;
+			if (col + k == in[i].target) v -= 1.0f - ls;
+			g[k] = in[i].target >= 0 && col + k < V ? v : 0.0f;
+		}
+		l[i] = make_float4(g[0], g[1], g[2], g[3]);
+		cs.x += g[0];
+		cs.y += g[1];
+		cs.z += g[2];
+		cs.w += g[3];
 	}
+	__syncthreads();                               // every logit of the block is in registers
+	unsigned char* out = reinterpret_cast<unsigned char*>(block);
+#pragma unroll
+	for (int i = 0; i < 8; ++i) {
+		const float4 v = make_float4(l[i].x * scale, l[i].y * scale, l[i].z * scale, l[i].w * scale);
+		const uint2 hi = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
+		unsigned char* dst = out + (r0 + 16 * i) * (kCols * 2) + q * 8;
+		*reinterpret_cast<uint2*>(dst) = hi;
+		if (two_parts) {
+			const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)),
+				h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+			*reinterpret_cast<uint2*>(dst + split16::kPartBytes) =
+				make_uint2(half2_bits(v.x - h0.x, v.y - h0.y), half2_bits(v.z - h1.x, v.w - h1.y));
+		}
+	}
+	if (!col_part) return;
+	// rows r0 and r0 + 1 of a warp, then the eight warps in order
+	cs.x += __shfl_xor_sync(0xffffffffu, cs.x, 16);
+	cs.y += __shfl_xor_sync(0xffffffffu, cs.y, 16);
+	cs.z += __shfl_xor_sync(0xffffffffu, cs.z, 16);
+	cs.w += __shfl_xor_sync(0xffffffffu, cs.w, 16);
+	if ((tid & 31) < 16) sums[tid >> 5][q] = cs;
 	__syncthreads();
-	ms = part[0];
-	total = part_s[0];
+	if (tid >= 64) return;
+	const float* f = reinterpret_cast<const float*>(sums);
+	float s = f[tid];
 #pragma unroll
-	for (int k = 1; k < kRowThreads / 32; ++k) {
-		ms = combine(ms, part[k]);
-		total += part_s[k];
-	}
-	// a row without a finite maximum (all -inf, or an infinity or NaN in it) has no softmax: NaN
-	if (!(ms.x > -INFINITY && ms.x < INFINITY)) ms.y = __int_as_float(0x7fc00000);
-	const float lt = row[t];
-	__syncthreads();                               // row[t] is read before its owner replaces it
-	if (threadIdx.x == 0) {
-		const float lse = logf(ms.y), nll = lse - (lt - ms.x);
-		row_loss[r] = ls == 0.0f ? nll : (1.0f - ls) * nll + ls * (lse - (total / (float)V - ms.x));
-		valid[r] = 1;
-	}
-	if (!grad) return;
-	const float inv = 1.0f / ms.y, spread = ls / (float)V;
-	for (int c = threadIdx.x; c < V; c += kRowThreads) {
-		float g = expf(row[c] - ms.x) * inv - spread;
-		if (c == t) g -= 1.0f - ls;
-		row[c] = g;
-	}
+	for (int k = 1; k < 8; ++k) s += f[k * 64 + tid];
+	col_part[(long long)rb * kw * kCols + c64 * kCols + tid] = s;
+}
+
+// db (+)= the row blocks' column sums, in order.
+__global__ void __launch_bounds__(128) ce_bias_kernel(const float* __restrict__ col_part, int row_blocks, int ld, int V,
+		float* __restrict__ db, int first) {
+	const int c = blockIdx.x * 128 + threadIdx.x;
+	if (c >= V) return;
+	float s = 0.0f;
+#pragma unroll 8
+	for (int k = 0; k < row_blocks; ++k) s += __ldg(col_part + (long long)k * ld + c);
+	db[c] = first ? s : db[c] + s;
 }
 
 // loss = sum of the row losses over their count, norm = 1 / count, in a fixed order in fp64.
@@ -157,12 +235,6 @@ __global__ void scaled_accumulate_kernel(long long n, const float* __restrict__ 
 	}
 }
 
-// Rows of one piece: as many whole 128-row tiles as keep its logits within kPieceBytes.
-long long piece_rows(long long rows, long long V) {
-	const long long fit = std::max<long long>(128, (long long)(kPieceBytes / sizeof(float)) / V / 128 * 128);
-	return std::min(rows, fit);
-}
-
 struct Call {
 	long long P, D, V, groups;
 	const float *x, *w, *bias;
@@ -171,32 +243,132 @@ struct Call {
 	float ls;
 	float *row_loss, *loss, *norm, *dx, *dw, *db;
 	long long dw_stride, db_stride;
+	bool grad() const { return dx || dw || db; }
+	long long parts() const { return 2 * ((V + split16::kBN - 1) / split16::kBN); }
+	long long kw() const { return (V + kCols - 1) / kCols; }
 };
 
-nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, float* logits, float* row_loss, int* valid) {
-	const int mode = math_mode();
-	const bool grad = c.dx || c.dw || c.db;
+// Rows of one piece of a group: whole 128-row blocks within the scratch limits, or 128.
+long long piece_rows(const Call& c) {
+	const long long per_row = c.grad() ? c.kw() * kCols * 4 : c.parts() * 8;
+	const long long limit = (long long)(c.grad() ? kPieceBytes : kPartBytes);
+	return std::min(c.P / c.groups, std::max<long long>(kRows, limit / per_row / kRows * kRows));
+}
+
+// The scratch buffer's parts, 1 KB aligned.
+struct Scratch {
+	size_t total = 0;
+	unsigned char* base = nullptr;
+	size_t take(size_t bytes) {
+		const size_t at = total;
+		total += (bytes + 1023) / 1024 * 1024;
+		return at;
+	}
+	template <typename T>
+	T* at(size_t off) const { return reinterpret_cast<T*>(base + off); }
+};
+
+struct Layout {
+	long long piece, blocks;                  // rows of a piece, and their 128-row blocks
+	int splits;                               // depth splits of dX
+	size_t ranges, wpack, xpack, x_bad, g, part, part_sum, target_logit, info, losses, valid, cols, slabs;
+};
+
+Layout plan(const Call& c, Scratch& s) {
+	Layout l;
+	l.piece = piece_rows(c);
+	l.blocks = (l.piece + kRows - 1) / kRows;
+	const size_t pad = (size_t)l.blocks * kRows;
+	l.splits = c.dx ? split16::choose_splits(l.piece, c.D, c.V) : 1;
+	l.ranges = s.take(2 * sizeof(split16::Range));
+	l.wpack = s.take(split16::pack_bytes(c.V, c.D));
+	l.xpack = s.take(split16::pack_bytes(l.piece, c.D));
+	l.x_bad = s.take(pad * sizeof(int));
+	l.g = s.take(c.grad() ? (size_t)l.blocks * c.kw() * kBlockBytes : 0);
+	l.part = s.take((size_t)c.parts() * pad * sizeof(float2));
+	l.part_sum = s.take(c.ls != 0.0f ? (size_t)c.parts() * pad * sizeof(float) : 0);
+	l.target_logit = s.take(pad * sizeof(float));
+	l.info = s.take(c.grad() ? pad * sizeof(RowInfo) : 0);
+	l.losses = s.take(c.row_loss ? 0 : (size_t)c.P * sizeof(float));
+	l.valid = s.take((size_t)c.P * sizeof(int));
+	l.cols = s.take(c.db ? (size_t)l.blocks * c.kw() * kCols * sizeof(float) : 0);
+	l.slabs = s.take(l.splits > 1 ? (size_t)l.splits * l.piece * c.D * sizeof(float) : 0);
+	return l;
+}
+
+nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l, const Scratch& m) {
+	const int parts = math_mode() == NNB_MATH_FP32X3 ? 2 : 1;
+	split16::Range* xr = m.at<split16::Range>(l.ranges);
+	split16::Range* wr = xr + 1;
+	float* row_loss = c.row_loss ? c.row_loss : m.at<float>(l.losses);
+	int* valid = m.at<int>(l.valid);
+	NNB_TRY(split16::find_range(s, c.x, c.P * c.D, xr));
+	NNB_TRY(split16::find_range(s, c.w, c.V * c.D, wr));
+	NNB_TRY(split16::pack(s, c.w, c.V, c.D, (c.V + 2 * kRows - 1) / (2 * kRows) * 2, parts, wr, m.at<void>(l.wpack), nullptr));
+	split16::Pack W, X, G;
+	W.buf = m.at<void>(l.wpack); W.rows = c.V; W.cols = c.D;
 	const long long rg = c.P / c.groups;             // parameter gradients are kept per group of rows
 	for (long long z = 0; z < c.groups; ++z) {
 		for (long long r0 = z * rg; r0 < (z + 1) * rg;) {
-			const long long n = std::min(piece_rows(rg, c.V), (z + 1) * rg - r0);
+			const long long n = std::min(l.piece, (z + 1) * rg - r0), blocks = (n + kRows - 1) / kRows, pad = blocks * kRows;
+			const int first = r0 == z * rg;
 			const float* x = c.x + r0 * c.D;
-			GemmDesc d;
-			d.tb = 1; d.m = n; d.n = c.V; d.k = c.D;
-			d.a = x; d.lda = c.D; d.b = c.w; d.ldb = c.D; d.c = logits; d.ldc = c.V; d.mode = mode;
-			d.epi.bias = c.bias; d.epi.bias_mode = c.bias ? kBiasCol : kBiasNone;
-			NNB_TRY(gemm_run(s, d));
+			int* x_bad = m.at<int>(l.x_bad);
+			NNB_CUDA_TRY(cudaMemsetAsync(x_bad, 0, (size_t)n * sizeof(int), s));
+			NNB_TRY(split16::pack(s, x, n, c.D, blocks, parts, xr, m.at<void>(l.xpack), x_bad));
+			X.buf = m.at<void>(l.xpack); X.rows = n; X.cols = c.D;
+
+			split16::Product p;
+			p.ra = xr; p.rb = wr;
+			p.bias = c.bias;
+			p.targets = c.targets + r0;
+			p.part = m.at<float2>(l.part);
+			p.part_sum = c.ls != 0.0f ? m.at<float>(l.part_sum) : nullptr;
+			p.target_logit = m.at<float>(l.target_logit);
+			if (c.grad()) {
+				p.blocks = m.at<float>(l.g);
+				p.blocks_kw = (int)c.kw();
+			}
+			NNB_TRY(split16::run(s, p, c.grad() ? split16::kLogits : split16::kStats, parts, X, false, W, false, n, c.V, c.D));
+			RowInfo* info = c.grad() ? m.at<RowInfo>(l.info) : nullptr;
 			{
 				TraceScope ts(s, kTraceRowwise);
-				ce_row_kernel<<<(unsigned)n, kRowThreads, 0, s>>>(logits, (int)c.V, c.targets + r0, c.ignore_index, c.ls, grad,
-					row_loss + r0, valid + r0, dev->error_word);
+				ce_rows_kernel<<<(unsigned)(pad / 32), 256, 0, s>>>(p.part, p.part_sum, p.target_logit, (int)c.parts(), (int)n,
+					(int)pad, (int)c.V, p.targets, c.ignore_index, c.ls, x_bad, wr, row_loss + r0, valid + r0, info,
+					dev->error_word);
 			}
-			NNB_TRY(cuda_status(cudaGetLastError(), "linear_ce row launch"));
-			const int first = r0 == z * rg;
-			if (c.dx || c.dw)
-				NNB_TRY(linear_bwd_gemms(s, n, c.D, c.V, 1, logits, x, nullptr, mode, c.w, c.dx ? c.dx + r0 * c.D : nullptr, 1,
-					c.dw ? c.dw + z * c.dw_stride : nullptr, 0, first));
-			if (c.db) NNB_TRY(colsum(s, logits, n, c.V, c.db + z * c.db_stride, first));
+			NNB_TRY(cuda_status(cudaGetLastError(), "linear_ce rows launch"));
+			if (c.grad()) {
+				float* cols = c.db ? m.at<float>(l.cols) : nullptr;
+				{
+					TraceScope ts(s, kTraceRowwise);
+					ce_grad_kernel<<<dim3((unsigned)c.kw(), (unsigned)blocks), 256, 0, s>>>(p.blocks, (int)c.kw(), (int)c.V, (int)pad,
+						info, c.ls, parts == 2, cols);
+				}
+				if (c.db) {
+					TraceScope ts(s, kTraceRowwise);
+					ce_bias_kernel<<<(unsigned)((c.V + 127) / 128), 128, 0, s>>>(cols, (int)blocks, (int)(c.kw() * kCols), (int)c.V,
+						c.db + z * c.db_stride, first);
+				}
+				NNB_TRY(cuda_status(cudaGetLastError(), "linear_ce gradient launch"));
+				G.buf = m.at<void>(l.g); G.rows = n; G.cols = c.V;
+			}
+			if (c.dx) {                                    // dX = G W
+				split16::Product d;
+				d.rb = wr; d.shift = kGShift;
+				float* out = c.dx + r0 * c.D;
+				d.splits = std::min(l.splits, split16::choose_splits(n, c.D, c.V));
+				d.C = d.splits > 1 ? m.at<float>(l.slabs) : out;
+				d.ldc = c.D; d.slab = d.splits > 1 ? n * c.D : 0;
+				NNB_TRY(split16::run(s, d, split16::kStore, parts, G, false, W, true, n, c.D, c.V));
+				if (d.splits > 1) NNB_TRY(split16::sum_slabs(s, d.C, d.splits, n * c.D, out, 0));
+			}
+			if (c.dw) {                                    // dW (+)= G^T X
+				split16::Product d;
+				d.rb = xr; d.shift = kGShift;
+				d.C = c.dw + z * c.dw_stride; d.ldc = c.D; d.accumulate = !first;
+				NNB_TRY(split16::run(s, d, split16::kStore, parts, G, true, X, true, c.V, c.D, n));
+			}
 			r0 += n;
 		}
 	}
@@ -237,13 +409,12 @@ nnb_status nnb_linear_ce_fwd(void* stream, size_t P, size_t D, size_t V, size_t 
 	c.row_loss = row_loss; c.loss = loss; c.norm = norm; c.dx = dx; c.dw = dw; c.db = db;
 	c.dw_stride = (long long)(dw_stride ? dw_stride : V * D);
 	c.db_stride = (long long)(db_stride ? db_stride : V);
-	const long long n = piece_rows(c.P / c.groups, c.V);
-	const size_t logits_bytes = ((size_t)n * V * sizeof(float) + 255) / 256 * 256;
+	Scratch m;
+	const Layout l = plan(c, m);
 	void* ws = nullptr;
-	NNB_TRY(scratch_alloc(&ws, logits_bytes + P * (sizeof(float) + sizeof(int)), s));
-	float* losses = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + logits_bytes);
-	const nnb_status st = run(s, c, dev, static_cast<float*>(ws), row_loss ? row_loss : losses,
-		reinterpret_cast<int*>(losses + P));
+	NNB_TRY(scratch_alloc(&ws, m.total, s));
+	m.base = static_cast<unsigned char*>(ws);
+	const nnb_status st = run(s, c, dev, l, m);
 	const nnb_status st2 = scratch_free(ws, s);
 	return st != NNB_OK ? st : st2;
 }

@@ -1,0 +1,557 @@
+// split16.cu -- the fp16-split product (nnb_split16.cuh): range, pack and the tcgen05 kernel.
+//
+// The kernel is warp-specialised, one CTA per SM, 12 warps:
+//   warp 0     TMA producer: a stage holds a 32-deep k-block, A 128 and B 256 rows (or columns), hi[, lo];
+//   warp 1     MMA issuer: kind::f16 128 x 256 x 16 into two TMEM accumulators in turn, one accumulator per
+//              chunk of 128 terms (3 x 8 MMAs);
+//   warps 4-11 epilogue: add each finished chunk into registers (128 columns per thread) while the tensor
+//              core works on the next, then store or reduce.
+// The 384 threads are launched with 168 registers each; warps 0-3 hand theirs down to 56 and the epilogue
+// takes 224 (4 x 32 x 56 + 8 x 32 x 224 = 384 x 168), which hold the 128 sums.
+// Tensor bound: 3 MMAs per 128 x 256 x 16 step, 1.6 PFLOP/s of fp16 (the measured bf16 burst rate) or 540
+// TFLOP/s of the fp32 product.
+#include <algorithm>
+#include <mutex>
+
+#include "nnb_ops.h"
+#include "nnb_split16.cuh"
+#include "nnb_trace.h"
+
+namespace nnb {
+namespace split16 {
+
+namespace {
+
+// ---- range and pack --------------------------------------------------------------------------
+
+__global__ void __launch_bounds__(256) range_kernel(const float* __restrict__ x, long long n, int vec, Range* out) {
+	unsigned top = 0, bad = 0;
+	auto see = [&](float v) {
+		const unsigned b = __float_as_uint(v) & 0x7fffffffu;
+		if (b >= 0x7f800000u) bad = 1;
+		else top = max(top, b);
+	};
+	const long long step = (long long)gridDim.x * blockDim.x;
+	long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
+	if (vec) {
+		const float4* x4 = reinterpret_cast<const float4*>(x);
+#pragma unroll 4
+		for (; i < n / 4; i += step) {
+			const float4 v = __ldg(x4 + i);
+			see(v.x);
+			see(v.y);
+			see(v.z);
+			see(v.w);
+		}
+	} else {
+#pragma unroll 4
+		for (; i < n; i += step) see(__ldg(x + i));
+	}
+	top = __reduce_max_sync(0xffffffffu, top);
+	bad = __reduce_or_sync(0xffffffffu, bad);
+	if ((threadIdx.x & 31) == 0) {                 // a maximum: the order does not matter
+		if (top) atomicMax(&out->top, top);
+		if (bad) atomicOr(&out->bad, 1u);
+	}
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+	const __half2 h = __floats2half2_rn(a, b);
+	return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four columns per thread: a float4 in (or four floats), 8 bytes of hi and of lo out.
+__global__ void __launch_bounds__(256) pack_kernel(const float* __restrict__ x, long long rows, long long cols, long long kw,
+		long long total, int vec, int parts, const Range* __restrict__ range, unsigned char* __restrict__ out,
+		int* __restrict__ row_bad) {
+	const float s = exp2_int(range_shift(range));
+	const long long quads = kw * (kCols / 4);
+	for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+		long long r, q;
+		if (total < 0x7fffffffLL) {
+			r = (unsigned)i / (unsigned)quads;
+			q = (unsigned)i - (unsigned)r * (unsigned)quads;
+		} else {
+			r = i / quads;
+			q = i - r * quads;
+		}
+		const long long c = q * 4;
+		float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+		if (r < rows && c < cols) {
+			const float* src = x + r * cols + c;
+			if (vec) {
+				const float4 t = __ldg(reinterpret_cast<const float4*>(src));
+				v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+			} else {
+#pragma unroll
+				for (int k = 0; k < 4; ++k)
+					if (c + k < cols) v[k] = __ldg(src + k);
+			}
+		}
+		bool bad = false;
+		float hi[4];
+#pragma unroll
+		for (int k = 0; k < 4; ++k) {
+			if (!isfinite(v[k])) {
+				bad = true;
+				v[k] = 0.0f;
+			}
+			v[k] *= s;
+			hi[k] = __half2float(__float2half_rn(v[k]));
+		}
+		if (bad && row_bad) row_bad[r] = 1;            // every writer writes 1
+		unsigned char* dst = out + ((r >> 7) * kw + (c >> 6)) * kBlockBytes + (r & 127) * (kCols * 2) + (c & 63) * 2;
+		*reinterpret_cast<uint2*>(dst) = make_uint2(half2_bits(hi[0], hi[1]), half2_bits(hi[2], hi[3]));
+		if (parts == 2)
+			*reinterpret_cast<uint2*>(dst + kPartBytes) =
+				make_uint2(half2_bits(v[0] - hi[0], v[1] - hi[1]), half2_bits(v[2] - hi[2], v[3] - hi[3]));
+	}
+}
+
+// ---- tcgen05 kind::f16 -----------------------------------------------------------------------
+
+// Instruction descriptor: fp32 accumulator, fp16 A and B.
+constexpr uint32_t idesc_f16(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+// MN-major 16-bit operand in the 128-byte swizzle: a row of 128 bytes holds 64 consecutive M (or N) elements
+// of one k; 8 k-rows form a 1024-byte group (stride byte offset to the next), and the next 64 elements sit
+// `lbo` bytes further on. One MMA (K = 16) reads two groups.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t lbo) {
+	uint64_t d = 0;
+	d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
+	d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
+	d |= (uint64_t)(1024u >> 4) << 32;
+	d |= (uint64_t)1 << 46;
+	d |= (uint64_t)2 << 61;                        // SWIZZLE_128B
+	return d;
+}
+
+// mma_tf32_elect's counterpart: the whole warp executes it, one lane issues.
+__device__ __forceinline__ void mma_f16_elect(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+	asm volatile(
+		"{\n\t.reg .pred p, e;\n\t"
+		"elect.sync _|e, 0xffffffff;\n\t"
+		"setp.ne.b32 p, %4, 0;\n\t"
+		"@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+		"l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+		: "memory");
+}
+
+constexpr int kGroupM = 16;                      // row tiles walked together, for L2 reuse of B
+constexpr int kAPart = kBM * kBK * 2, kBPart = kBN * kBK * 2;
+constexpr int kEpiTile = 32 * 32 * 4;            // staging tile of one epilogue warp
+__host__ __device__ constexpr int stage_bytes(int parts) { return parts * (kAPart + kBPart); }
+__host__ __device__ constexpr int stages(int parts) { return 4 * 2 / parts; }
+__host__ __device__ constexpr int smem_bytes(int parts) {
+	return stages(parts) * stage_bytes(parts) + kEpiWarps * kEpiTile + 1024;
+}
+
+struct Item {
+	int mt, nt, split, kb0, kb1;
+};
+// Item t: tiles in groups of kGroupM row tiles, all splits of a tile together.
+__device__ __forceinline__ Item item_at(int t, const Product& p) {
+	Item it;
+	it.split = t % p.splits;
+	const int tile = t / p.splits;
+	const int group = tile / (kGroupM * p.tiles_n), first = group * kGroupM, size = min(p.tiles_m - first, kGroupM);
+	const int in = tile - group * kGroupM * p.tiles_n;
+	it.mt = first + in % size;
+	it.nt = in / size;
+	it.kb0 = it.split * p.split_kb;
+	it.kb1 = min(p.kb, it.kb0 + p.split_kb);
+	return it;
+}
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+template <int kParts, bool kMnA, bool kMnB, int kEpi>
+__global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_constant__ CUtensorMap tm_a,
+		const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ Product p) {
+	constexpr int kStages = stages(kParts), kStageBytes = stage_bytes(kParts);
+	extern __shared__ uint8_t smem_raw[];
+	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+	__shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], accf_bar[2], acce_bar[2];
+	__shared__ uint32_t tmem_base_sh;
+	__shared__ int abort_sh;
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	if (threadIdx.x == 0) {
+		for (int s = 0; s < kStages; ++s) {
+			mbar_init(smem_u32(&full_bar[s]), 1);
+			mbar_init(smem_u32(&empty_bar[s]), 1);
+		}
+		for (int b = 0; b < 2; ++b) {
+			mbar_init(smem_u32(&accf_bar[b]), 1);
+			mbar_init(smem_u32(&acce_bar[b]), kEpiWarps);
+		}
+		abort_sh = 0;
+		fence_mbar_init();
+		tma_prefetch_desc(&tm_a);
+		tma_prefetch_desc(&tm_b);
+	}
+	if (warp == 1) {
+		tmem_alloc(smem_u32(&tmem_base_sh), 2 * kBN);
+		tmem_relinquish();
+	}
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	const uint32_t tmem_base = tmem_base_sh;
+	volatile int* abort_flag = &abort_sh;
+	const int items = p.tiles_m * p.tiles_n * p.splits;
+	static_assert(128 * 56 + 32 * kEpiWarps * 224 <= kThreads * 168, "registers handed over");
+
+	if (warp < 4) {
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+		if (warp == 0 && lane == 0) {
+			// ------------------------------ TMA producer ------------------------------
+			int stage = 0;
+			uint32_t phase = 0;
+			bool ok = true;
+			for (int t = blockIdx.x; ok && t < items; t += gridDim.x) {
+				const Item it = item_at(t, p);
+				for (int kb = it.kb0; kb < it.kb1; ++kb) {
+					if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, p.err, kDevTimeoutEmpty, abort_flag)) {
+						ok = false;
+						break;
+					}
+					const uint32_t fb = smem_u32(&full_bar[stage]);
+					mbar_arrive_expect_tx(fb, kStageBytes);
+					const uint32_t base = smem_u32(smem + stage * kStageBytes);
+#pragma unroll
+					for (int s = 0; s < kParts; ++s) {
+						// K-major: half a block's 128-byte rows (32 of its 64 columns); MN-major: 32 of a block
+						// row's 128 rows, 64 columns per chunk. Coordinates count 4-byte units.
+						if (kMnA)
+							tma_load_5d(base + s * kAPart, &tm_a, fb, 0, (kb & 3) * kBK, s, it.mt * (kBM / kCols), kb >> 2);
+						else
+							tma_load_2d(base + s * kAPart, &tm_a, fb, (kb & 1) * (kBK / 2),
+								((it.mt * p.a_kw + (kb >> 1)) * 2 + s) * kRows);
+						const uint32_t bb = base + kParts * kAPart + s * kBPart;
+						if (kMnB) {
+							tma_load_5d(bb, &tm_b, fb, 0, (kb & 3) * kBK, s, it.nt * (kBN / kCols), kb >> 2);
+						} else {
+#pragma unroll
+							for (int q = 0; q < 2; ++q)
+								tma_load_2d(bb + q * (kBPart / 2), &tm_b, fb, (kb & 1) * (kBK / 2),
+									(((it.nt * 2 + q) * p.b_kw + (kb >> 1)) * 2 + s) * kRows);
+						}
+					}
+					if (++stage == kStages) {
+						stage = 0;
+						phase ^= 1;
+					}
+				}
+			}
+		} else if (warp == 1) {
+			// --------------------- MMA issuer (the whole warp; one elected lane issues) ---------------------
+			constexpr uint32_t idesc = idesc_f16(kBM, kBN) | (kMnA ? kIdescAMajorMN : 0u) | (kMnB ? kIdescBMajorMN : 0u);
+			int stage = 0;
+			uint32_t phase = 0;
+			int v = 0;                                     // chunks so far: accumulator v & 1
+			bool ok = true;
+			for (int t = blockIdx.x; ok && t < items; t += gridDim.x) {
+				const Item it = item_at(t, p);
+				for (int c0 = it.kb0; ok && c0 < it.kb1; c0 += kChunkKb, ++v) {
+					if (!mbar_wait_warp(smem_u32(&acce_bar[v & 1]), ((v >> 1) & 1) ^ 1, p.err, kDevTimeoutAccumFree, abort_flag)) {
+						ok = false;
+						break;
+					}
+					tc_fence_after();
+					const uint32_t d = tmem_base + (v & 1) * kBN;
+					const int c1 = min(it.kb1, c0 + kChunkKb);
+					for (int kb = c0; kb < c1; ++kb) {
+						if (!mbar_wait_warp(smem_u32(&full_bar[stage]), phase, p.err, kDevTimeoutFull, abort_flag)) {
+							ok = false;
+							break;
+						}
+						tc_fence_after();
+						const uint32_t a0 = smem_u32(smem + stage * kStageBytes), b0 = a0 + kParts * kAPart;
+	#pragma unroll
+						for (int kk = 0; kk < kBK / 16; ++kk) {
+							// 16 deep: 32 bytes along a K-major row, or 16 rows of 128 bytes
+							auto desc = [&](bool mn, uint32_t addr) {
+								return mn ? smem_desc_mn_sw128(addr + kk * 2048, kBK * 128) : smem_desc_k_sw64(addr + kk * 32);
+							};
+							const uint64_t a_hi = desc(kMnA, a0), b_hi = desc(kMnB, b0);
+							const uint32_t more = (kb > c0 || kk > 0) ? 1u : 0u;
+							if (kParts == 2) {
+								const uint64_t a_lo = desc(kMnA, a0 + kAPart), b_lo = desc(kMnB, b0 + kBPart);
+								mma_f16_elect(d, a_lo, b_hi, idesc, more);
+								mma_f16_elect(d, a_hi, b_lo, idesc, 1u);
+								mma_f16_elect(d, a_hi, b_hi, idesc, 1u);
+							} else {
+								mma_f16_elect(d, a_hi, b_hi, idesc, more);
+							}
+						}
+						mma_commit_elect(smem_u32(&empty_bar[stage]));
+						if (++stage == kStages) {
+							stage = 0;
+							phase ^= 1;
+						}
+					}
+					if (ok) mma_commit_elect(smem_u32(&accf_bar[v & 1]));
+				}
+			}
+		}
+	} else {
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+		// ---------------------------------- epilogue ----------------------------------
+		const int quad = warp & 3, half = (warp - 4) >> 2;   // TMEM lanes and columns of this warp
+		const int row = quad * 32 + lane;
+		float* stage = reinterpret_cast<float*>(smem + (size_t)kStages * kStageBytes + (warp - 4) * kEpiTile);
+		float4* st4 = reinterpret_cast<float4*>(stage);
+		float alpha_a = exp2_int(-p.shift), alpha_b = 1.0f;
+		if (p.ra) alpha_a *= exp2_int(-range_shift(p.ra));
+		if (p.rb) alpha_b = exp2_int(-range_shift(p.rb));
+		const bool vec_ok = kEpi == kStore && p.ldc % 4 == 0 && p.slab % 4 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15) == 0;
+		int v = 0;
+		bool ok = true;
+		for (int t = blockIdx.x; ok && t < items; t += gridDim.x) {
+			const Item it = item_at(t, p);
+			float acc[kBN / 2];
+#pragma unroll
+			for (int j = 0; j < kBN / 2; ++j) acc[j] = 0.0f;
+			for (int c0 = it.kb0; c0 < it.kb1; c0 += kChunkKb, ++v) {
+				if (!mbar_wait_warp(smem_u32(&accf_bar[v & 1]), (v >> 1) & 1, p.err, kDevTimeoutAccum, abort_flag)) {
+					ok = false;
+					break;
+				}
+				tc_fence_after();
+				const uint32_t src = tmem_base + ((uint32_t)(quad * 32) << 16) + (v & 1) * kBN + half * (kBN / 2);
+#pragma unroll
+				for (int c = 0; c < kBN / 32; ++c) {
+					uint32_t r[16];
+					tmem_ld_32x32b_x16(src + c * 16, r);
+					tmem_wait_ld();
+#pragma unroll
+					for (int j = 0; j < 16; ++j) acc[c * 16 + j] += __uint_as_float(r[j]);
+				}
+				tc_fence_before();
+				__syncwarp();
+				if (lane == 0) mbar_arrive(smem_u32(&acce_bar[v & 1]));
+			}
+			if (!ok) break;
+			const int gm = it.mt * kBM + row, n0 = it.nt * kBN + half * (kBN / 2);
+			// the warp's 32 x 32 values (row per lane) to rows dst + r * ld, as 128-byte row segments: through the
+			// staging tile, element (r, c) at float4 r * 8 + (c / 4 ^ r % 8), without bank conflicts either way
+			auto stage_rows = [&](float* dst, long long ld, int rows, int c, bool add) {
+#pragma unroll
+				for (int g = 0; g < 8; ++g)
+					st4[lane * 8 + (g ^ (lane & 7))] =
+						make_float4(acc[c * 32 + 4 * g], acc[c * 32 + 4 * g + 1], acc[c * 32 + 4 * g + 2], acc[c * 32 + 4 * g + 3]);
+				__syncwarp();
+				const int g = lane & 7;
+#pragma unroll
+				for (int k = 0; k < 8; ++k) {
+					const int rr = 4 * k + (lane >> 3);
+					float4 o = st4[rr * 8 + (g ^ (rr & 7))];
+					if (rr < rows) {
+						float4* d4 = reinterpret_cast<float4*>(dst + rr * ld) + g;
+						if (add) {
+							const float4 old = *d4;
+							o = make_float4(old.x + o.x, old.y + o.y, old.z + o.z, old.w + o.w);
+						}
+						*d4 = o;
+					}
+				}
+				__syncwarp();
+			};
+			const int warp_row = it.mt * kBM + quad * 32, rows_here = max(0, min(32, p.M - warp_row));
+			if (kEpi == kStore) {
+				float* C = p.C + it.split * p.slab;
+#pragma unroll
+				for (int c = 0; c < kBN / 64; ++c) {
+					const int gn = n0 + c * 32;
+					if (gn >= p.N) break;                  // warp-uniform
+#pragma unroll
+					for (int j = 0; j < 32; ++j) acc[c * 32 + j] = acc[c * 32 + j] * alpha_a * alpha_b;
+					if (vec_ok && gn + 32 <= p.N) {
+						stage_rows(C + (long long)warp_row * p.ldc + gn, p.ldc, rows_here, c, p.accumulate != 0);
+					} else if (gm < p.M) {
+						float* dst = C + (long long)gm * p.ldc + gn;
+#pragma unroll
+						for (int j = 0; j < 32; ++j)
+							if (gn + j < p.N) dst[j] = p.accumulate ? dst[j] + acc[c * 32 + j] : acc[c * 32 + j];
+					}
+				}
+			} else {
+				const int64_t target = gm < p.M ? p.targets[gm] : -1;
+				const int tj = target >= n0 && target < n0 + kBN / 2 && target < p.N ? (int)(target - n0) : -1;
+				float top = -INFINITY, total = 0.0f, at = 0.0f;
+#pragma unroll
+				for (int j = 0; j < kBN / 2; ++j) {
+					const bool in = n0 + j < p.N;          // warp-uniform
+					const float l = acc[j] * alpha_a * alpha_b + (in && p.bias ? __ldg(p.bias + n0 + j) : 0.0f);
+					acc[j] = l;
+					if (in) {
+						top = fmaxf(top, l);
+						total += l;
+					}
+					if (j == tj) at = l;
+				}
+				float sum = 0.0f;
+#pragma unroll
+				for (int j = 0; j < kBN / 2; ++j)
+					if (n0 + j < p.N) sum += exp2_hw((acc[j] - top) * kLog2e);
+				if (top == -INFINITY && sum != sum) sum = total != total ? total : 0.0f;   // all -inf: an empty part
+				const long long slot = (long long)(it.nt * 2 + half) * (p.tiles_m * kBM) + gm;
+				p.part[slot] = make_float2(top, sum);
+				if (p.part_sum) p.part_sum[slot] = total;
+				if (tj >= 0) p.target_logit[gm] = at;
+				if (kEpi == kLogits) {
+#pragma unroll
+					for (int c = 0; c < kBN / 64; ++c) {
+						const int gn = n0 + c * 32;
+						if (gn >= p.blocks_kw * kCols) break;
+						stage_rows(p.blocks + ((long long)it.mt * p.blocks_kw + gn / kCols) * (kRows * kCols) + quad * 32 * kCols +
+							gn % kCols, kCols, 32, c, false);
+					}
+				}
+			}
+		}
+	}
+	tc_fence_before();
+	__syncthreads();
+	if (warp == 1) {
+		__syncwarp();
+		tc_fence_after();
+		tmem_dealloc(tmem_base, 2 * kBN);
+	}
+}
+
+// c (+)= sum over slabs, in order; four floats per thread where aligned.
+__global__ void __launch_bounds__(256) sum_slabs_kernel(const float* __restrict__ slabs, int splits, long long n,
+		float* __restrict__ c, int accumulate, int vec) {
+	const long long step = gridDim.x * 256LL;
+	long long i = blockIdx.x * 256LL + threadIdx.x;
+	if (vec) {
+		for (; i < n / 4; i += step) {
+			float4 a = __ldg(reinterpret_cast<const float4*>(slabs) + i);
+#pragma unroll 4
+			for (int k = 1; k < splits; ++k) {
+				const float4 b = __ldg(reinterpret_cast<const float4*>(slabs + k * n) + i);
+				a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+			}
+			float4* d = reinterpret_cast<float4*>(c) + i;
+			if (accumulate) {
+				const float4 o = *d;
+				a = make_float4(o.x + a.x, o.y + a.y, o.z + a.z, o.w + a.w);
+			}
+			*d = a;
+		}
+	} else {
+		for (; i < n; i += step) {
+			float a = __ldg(slabs + i);
+			for (int k = 1; k < splits; ++k) a += __ldg(slabs + k * n + i);
+			c[i] = accumulate ? c[i] + a : a;
+		}
+	}
+}
+
+// Tensor map of a pack read K-major: its 128-byte rows as 32 4-byte units, half a row per box.
+nnb_status map_k(CUtensorMap* map, const Pack& a, long long row_blocks) {
+	const long long rows = row_blocks * a.kw() * 2 * kRows;
+	if (rows > INT32_MAX) return fail(NNB_ERR_UNSUPPORTED, "split product: operand too large");
+	return encode_tiled_2d(map, a.buf, kCols / 2, (uint64_t)rows, kCols * 2, kBK / 2, kRows, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+// The same read MN-major: (64 columns, 128 rows, part, packed column, row block), boxes of 32 rows and
+// `chunks` packed columns.
+nnb_status map_mn(CUtensorMap* map, const Pack& a, int chunks) {
+	const uint64_t kw = (uint64_t)a.kw();
+	const uint64_t dims[5] = {kCols / 2, kRows, 2, kw, (uint64_t)a.row_blocks()};
+	const uint64_t strides[4] = {kCols * 2, kPartBytes, kBlockBytes, kw * kBlockBytes};
+	const uint32_t box[5] = {kCols / 2, kBK, 1, (uint32_t)chunks, 1};
+	return encode_tiled_nd(map, a.buf, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int kParts, bool kMnA, bool kMnB, int kEpi>
+nnb_status launch(cudaStream_t s, const DeviceState* dev, const Product& p, const CUtensorMap& ta, const CUtensorMap& tb) {
+	auto kernel = split16_kernel<kParts, kMnA, kMnB, kEpi>;
+	NNB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kParts)));
+	const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
+	{
+		TraceScope ts(s, kTraceGemm);
+		kernel<<<(unsigned)std::min<long long>(items, dev->sm_count), kThreads, smem_bytes(kParts), s>>>(ta, tb, p);
+	}
+	return cuda_status(cudaGetLastError(), "split product launch");
+}
+
+template <int kParts>
+nnb_status dispatch(cudaStream_t s, const DeviceState* dev, int epilogue, bool mn_a, bool mn_b, const Product& p,
+		const CUtensorMap& ta, const CUtensorMap& tb) {
+	if (epilogue == kStats && !mn_a && !mn_b) return launch<kParts, false, false, kStats>(s, dev, p, ta, tb);
+	if (epilogue == kLogits && !mn_a && !mn_b) return launch<kParts, false, false, kLogits>(s, dev, p, ta, tb);
+	if (epilogue == kStore && !mn_a && mn_b) return launch<kParts, false, true, kStore>(s, dev, p, ta, tb);
+	if (epilogue == kStore && mn_a && mn_b) return launch<kParts, true, true, kStore>(s, dev, p, ta, tb);
+	return fail(NNB_ERR_UNSUPPORTED, "split product: form not built");
+}
+
+}  // namespace
+
+nnb_status find_range(cudaStream_t s, const float* x, long long n, Range* out) {
+	NNB_CUDA_TRY(cudaMemsetAsync(out, 0, sizeof(Range), s));
+	const bool vec = n % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+	{
+		TraceScope ts(s, kTracePack);
+		range_kernel<<<(unsigned)std::min<long long>((n + 4095) / 4096, 148 * 8), 256, 0, s>>>(x, n, vec, out);
+	}
+	return cuda_status(cudaGetLastError(), "range launch");
+}
+
+nnb_status pack(cudaStream_t s, const float* x, long long rows, long long cols, long long row_blocks, int parts,
+		const Range* range, void* buf, int* row_bad) {
+	const long long kw = (cols + kCols - 1) / kCols, total = row_blocks * kRows * kw * (kCols / 4);
+	const bool vec = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+	{
+		TraceScope ts(s, kTracePack);
+		pack_kernel<<<(unsigned)std::min<long long>((total + 255) / 256, 148 * 32), 256, 0, s>>>(x, rows, cols, kw, total, vec,
+			parts, range, static_cast<unsigned char*>(buf), row_bad);
+	}
+	return cuda_status(cudaGetLastError(), "split pack launch");
+}
+
+int choose_splits(long long M, long long N, long long K) {
+	// A product with fewer tiles than SMs is cut along its depth until two waves of items are there, in
+	// pieces of whole chunks and at least 1024 terms
+	const long long tiles = (M + kBM - 1) / kBM * ((N + kBN - 1) / kBN), chunks = (K + kBK * kChunkKb - 1) / (kBK * kChunkKb);
+	if (tiles >= 148) return 1;
+	const long long want = std::max<long long>(1, std::min<long long>(2 * 148 / tiles, chunks / 8)), per = (chunks + want - 1) / want;
+	return (int)((chunks + per - 1) / per);
+}
+
+nnb_status run(cudaStream_t s, Product p, int epilogue, int parts, const Pack& a, bool mn_a, const Pack& b, bool mn_b,
+		long long M, long long N, long long K) {
+	DeviceState* dev = nullptr;
+	NNB_TRY(device_state(&dev));
+	p.M = (int)M;
+	p.N = (int)N;
+	p.kb = (int)((K + kBK - 1) / kBK);
+	p.tiles_m = (int)((M + kBM - 1) / kBM);
+	p.tiles_n = (int)((N + kBN - 1) / kBN);
+	if ((long long)p.tiles_m * p.tiles_n * p.splits > INT32_MAX) return fail(NNB_ERR_UNSUPPORTED, "split product: too many tiles");
+	// whole chunks per split, and no empty split
+	p.split_kb = ((p.kb + p.splits - 1) / p.splits + kChunkKb - 1) / kChunkKb * kChunkKb;
+	if ((p.kb + p.split_kb - 1) / p.split_kb != p.splits) return fail(NNB_ERR_INVALID, "split product: empty depth split");
+	p.a_kw = (int)a.kw();
+	p.b_kw = (int)b.kw();
+	p.err = dev->error_word;
+	CUtensorMap ta, tb;
+	if (mn_a) NNB_TRY(map_mn(&ta, a, kBM / kCols));
+	else NNB_TRY(map_k(&ta, a, a.row_blocks()));
+	if (mn_b) NNB_TRY(map_mn(&tb, b, kBN / kCols));
+	else NNB_TRY(map_k(&tb, b, (b.row_blocks() + 1) / 2 * 2));      // a 256-row tile reads whole pairs of blocks
+	return parts == 2 ? dispatch<2>(s, dev, epilogue, mn_a, mn_b, p, ta, tb) : dispatch<1>(s, dev, epilogue, mn_a, mn_b, p, ta, tb);
+}
+
+nnb_status sum_slabs(cudaStream_t s, const float* slabs, int splits, long long n, float* c, int accumulate) {
+	const bool vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(slabs) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
+	{
+		TraceScope ts(s, kTraceAux);
+		sum_slabs_kernel<<<grid_for(vec ? n / 4 : n, 256), 256, 0, s>>>(slabs, splits, n, c, accumulate, vec);
+	}
+	return cuda_status(cudaGetLastError(), "slab sum launch");
+}
+
+}  // namespace split16
+}  // namespace nnb

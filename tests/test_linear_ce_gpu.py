@@ -1,10 +1,13 @@
 """The vocabulary projection's loss and gradients against their definition in 64 bits.
 
-E = 2^-24 is half a step of fp32. The bounds start from the product's: in 3xTF32 an operand's two parts
-leave out 2^-22 of it, so a product of K terms is off by at most
-  g(K) = 2^-21 + (3 ceil(K / 8) + 4) 2^-23       times the sum of the terms' magnitudes
-(the operands' parts and the dropped product of their low parts, then one accumulation of at most one part
-in 2^23 per tensor-core step of 8, and the partial sums of a depth cut).
+E = 2^-24 is half a step of fp32. The bounds start from the product's. An operand goes in as two fp16 parts
+of 11 bits: they leave out 2^-22 of a value, or 2^-39 of the matrix' largest magnitude where the value is
+below 2^-17 of it (half of the last step 2^-24 of a part, the largest being scaled to 2^14 at least; G,
+at most 1, is scaled by 2^15: 2^-40). The product of the low parts is left out, another 2^-22. The tensor
+core adds 128 terms in 24 additions, each off by at most one part in 2^23 of the magnitudes; those sums
+are then added in fp32. So a product of K terms is off by at most
+  g(K) = 3 2^-22 + min(24, 3 ceil(K / 16)) 2^-23 + (ceil(K / 128) + 2) 2^-24
+times the sum of the terms' magnitudes, and what the small values' absolute errors add.
 """
 import math
 
@@ -23,7 +26,7 @@ IGNORE = -100
 
 
 def g(K):
-    return 2.0 ** -21 + (3 * math.ceil(K / 8) + 4) * 2.0 ** -23
+    return 3 * 2.0 ** -22 + min(24, 3 * math.ceil(K / 16)) * 2.0 ** -23 + (math.ceil(K / 128) + 2) * 2.0 ** -24
 
 
 def _make(P, D, V, bias=True, ignored=0.0, seed=0, shift=0):
@@ -49,6 +52,7 @@ def _want(x, w, b, t, ls, up=1.0, norm=None):
     l = x @ w.t() + bias
     # logits: the product, and the bias' addition (1 rounding)
     el = g(D) * (x.abs() @ w.abs().t()) + E * l.abs() * 2
+    el += 2.0 ** -39 * (float(x.abs().max()) * w.abs().sum(1) + float(w.abs().max()) * x.abs().sum(1)[:, None])
     live = t != IGNORE
     at = t.clamp(min=0)[:, None]
     lse = torch.logsumexp(l, 1)
@@ -68,10 +72,13 @@ def _want(x, w, b, t, ls, up=1.0, norm=None):
     G = (p - q) * mask
     # p: twice the worst logit, the sum's roundings, exponential, argument, quotient; then the subtractions
     eG = mask * (p * (2 * worst[:, None] + sums + 8 * E + E * (l - l.amax(1, keepdim=True)).abs()) + 4 * E * q)
+    eG += 2.0 ** -40 * mask
+    small_w = 2.0 ** -39 * float(w.abs().max()) * G.abs().sum(1, keepdim=True)
+    small_x = 2.0 ** -39 * float(x.abs().max()) * G.abs().sum(0)[:, None]
     out = {"loss": (loss, eloss), "rows": (rows, erows)}
     for name, value, err in (
-            ("x", G @ w, eG @ w.abs() + g(V) * (G.abs() @ w.abs())),
-            ("w", G.t() @ x, eG.t() @ x.abs() + (g(min(P, 4096)) + (P / 128 + 2) * E) * (G.abs().t() @ x.abs())),
+            ("x", G @ w, eG @ w.abs() + g(V) * (G.abs() @ w.abs()) + small_w),
+            ("w", G.t() @ x, eG.t() @ x.abs() + g(P) * (G.abs().t() @ x.abs()) + small_x),
             ("b", G.sum(0), eG.sum(0) + (P + 8) * E * G.abs().sum(0))):
         out[name] = value * k, err * abs(k) + 4 * E * value.abs() * abs(k)
     return out
