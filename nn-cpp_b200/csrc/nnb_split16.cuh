@@ -101,8 +101,10 @@ nnb_status pack(cudaStream_t s, const float* x, long long rows, long long cols, 
 // widths and tile counts are filled in here. parts: 2 or 1.
 nnb_status run(cudaStream_t s, Product p, int epilogue, int parts, const Pack& a, bool mn_a, const Pack& b, bool mn_b,
 		long long M, long long N, long long K);
-// Depth splits that fill the GPU for an M x N product of depth K; depends on the sizes only.
+// Depth splits for an M x N product of depth K; depends on the sizes only.
 int choose_splits(long long M, long long N, long long K);
+// The splits, at most `want`, that cut a depth of K into whole chunks with none empty (Product::splits).
+int split_count(long long K, int want);
 // c (+)= sum over `splits` slabs of n floats, in order.
 nnb_status sum_slabs(cudaStream_t s, const float* slabs, int splits, long long n, float* c, int accumulate);
 

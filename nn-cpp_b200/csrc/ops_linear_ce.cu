@@ -43,14 +43,15 @@ struct RowInfo {
 	int unused;
 };
 
-// A row's statistics from its parts (32 rows per CTA, eight threads to a row), its loss and RowInfo.
+// A row's statistics from its parts (eight rows per CTA, 32 threads to a row: few rows must fill the GPU), its
+// loss and RowInfo.
 __global__ void __launch_bounds__(256) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ part_sum,
 		const float* __restrict__ target_logit, int parts, int rows, int rows_pad, int V, const int64_t* __restrict__ targets,
 		int64_t ignore_index, float ls, const int* __restrict__ x_bad, const split16::Range* __restrict__ w_range,
 		float* __restrict__ row_loss, int* __restrict__ valid, RowInfo* __restrict__ info, int* err) {
-	__shared__ float2 ms[8][32];
-	__shared__ float tot[8][32];
-	const int x = threadIdx.x & 31, y = threadIdx.x >> 5, r = blockIdx.x * 32 + x;
+	__shared__ float2 ms[32][9];
+	__shared__ float tot[32][9];
+	const int x = threadIdx.x & 7, y = threadIdx.x >> 3, r = blockIdx.x * 8 + x;
 	float top = -INFINITY, sum = 0.0f, total = 0.0f;
 	// (an empty part is (-inf, 0); a NaN or infinite logit leaves a NaN sum, and so does +inf as a maximum)
 	auto join = [&](float2 b) {
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const float2* __restrict__
 	};
 	if (r < rows)
 #pragma unroll 4
-		for (int k = y; k < parts; k += 8) {
+		for (int k = y; k < parts; k += 32) {
 			join(part[(long long)k * rows_pad + r]);
 			if (part_sum) total += part_sum[(long long)k * rows_pad + r];
 		}
@@ -74,8 +75,8 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const float2* __restrict__
 	if (y != 0 || r >= rows_pad) return;
 	RowInfo o = {0.0f, 0.0f, -1, 0};
 	if (r < rows) {
-#pragma unroll
-		for (int k = 1; k < 8; ++k) {
+#pragma unroll 4
+		for (int k = 1; k < 32; ++k) {
 			join(ms[k][x]);
 			total += tot[k][x];
 		}
@@ -166,14 +167,21 @@ __global__ void __launch_bounds__(256) ce_grad_kernel(float* __restrict__ blocks
 	col_part[(long long)rb * kw * kCols + c64 * kCols + tid] = s;
 }
 
-// db (+)= the row blocks' column sums, in order.
-__global__ void __launch_bounds__(128) ce_bias_kernel(const float* __restrict__ col_part, int row_blocks, int ld, int V,
+// db (+)= the row blocks' column sums: 32 columns per CTA, warp y sums blocks y, y + 8, ..., then the eight
+// sums in order.
+__global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ col_part, int row_blocks, int ld, int V,
 		float* __restrict__ db, int first) {
-	const int c = blockIdx.x * 128 + threadIdx.x;
-	if (c >= V) return;
+	__shared__ float tile[8][32];
+	const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
 	float s = 0.0f;
+	if (c < V)
 #pragma unroll 8
-	for (int k = 0; k < row_blocks; ++k) s += __ldg(col_part + (long long)k * ld + c);
+		for (int k = y; k < row_blocks; k += 8) s += __ldg(col_part + (long long)k * ld + c);
+	tile[y][lane] = s;
+	__syncthreads();
+	if (y != 0 || c >= V) return;
+#pragma unroll
+	for (int k = 1; k < 8; ++k) s += tile[k][lane];
 	db[c] = first ? s : db[c] + s;
 }
 
@@ -270,7 +278,7 @@ struct Scratch {
 
 struct Layout {
 	long long piece, blocks;                  // rows of a piece, and their 128-row blocks
-	int splits;                               // depth splits of dX
+	int dx_splits, dw_splits;                 // depth splits of the gradients' products
 	size_t ranges, wpack, xpack, x_bad, g, part, part_sum, target_logit, info, losses, valid, cols, slabs;
 };
 
@@ -279,7 +287,8 @@ Layout plan(const Call& c, Scratch& s) {
 	l.piece = piece_rows(c);
 	l.blocks = (l.piece + kRows - 1) / kRows;
 	const size_t pad = (size_t)l.blocks * kRows;
-	l.splits = c.dx ? split16::choose_splits(l.piece, c.D, c.V) : 1;
+	l.dx_splits = c.dx ? split16::choose_splits(l.piece, c.D, c.V) : 1;
+	l.dw_splits = c.dw ? split16::choose_splits(c.V, c.D, l.piece) : 1;
 	l.ranges = s.take(2 * sizeof(split16::Range));
 	l.wpack = s.take(split16::pack_bytes(c.V, c.D));
 	l.xpack = s.take(split16::pack_bytes(l.piece, c.D));
@@ -292,7 +301,8 @@ Layout plan(const Call& c, Scratch& s) {
 	l.losses = s.take(c.row_loss ? 0 : (size_t)c.P * sizeof(float));
 	l.valid = s.take((size_t)c.P * sizeof(int));
 	l.cols = s.take(c.db ? (size_t)l.blocks * c.kw() * kCols * sizeof(float) : 0);
-	l.slabs = s.take(l.splits > 1 ? (size_t)l.splits * l.piece * c.D * sizeof(float) : 0);
+	l.slabs = s.take(std::max(l.dx_splits > 1 ? (size_t)l.dx_splits * l.piece * c.D : 0,
+		l.dw_splits > 1 ? (size_t)l.dw_splits * c.V * c.D : 0) * sizeof(float));
 	return l;
 }
 
@@ -333,7 +343,7 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 			RowInfo* info = c.grad() ? m.at<RowInfo>(l.info) : nullptr;
 			{
 				TraceScope ts(s, kTraceRowwise);
-				ce_rows_kernel<<<(unsigned)(pad / 32), 256, 0, s>>>(p.part, p.part_sum, p.target_logit, (int)c.parts(), (int)n,
+				ce_rows_kernel<<<(unsigned)(pad / 8), 256, 0, s>>>(p.part, p.part_sum, p.target_logit, (int)c.parts(), (int)n,
 					(int)pad, (int)c.V, p.targets, c.ignore_index, c.ls, x_bad, wr, row_loss + r0, valid + r0, info,
 					dev->error_word);
 			}
@@ -347,28 +357,27 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 				}
 				if (c.db) {
 					TraceScope ts(s, kTraceRowwise);
-					ce_bias_kernel<<<(unsigned)((c.V + 127) / 128), 128, 0, s>>>(cols, (int)blocks, (int)(c.kw() * kCols), (int)c.V,
+					ce_bias_kernel<<<(unsigned)((c.V + 31) / 32), 256, 0, s>>>(cols, (int)blocks, (int)(c.kw() * kCols), (int)c.V,
 						c.db + z * c.db_stride, first);
 				}
 				NNB_TRY(cuda_status(cudaGetLastError(), "linear_ce gradient launch"));
 				G.buf = m.at<void>(l.g); G.rows = n; G.cols = c.V;
 			}
-			if (c.dx) {                                    // dX = G W
+			// a product cut along its depth leaves its pieces in slabs, summed in order
+			auto product = [&](const split16::Pack& a, bool mn_a, const split16::Pack& b, const split16::Range* rb, long long M,
+					long long K, int max_splits, float* out, int accumulate) -> nnb_status {
 				split16::Product d;
-				d.rb = wr; d.shift = kGShift;
-				float* out = c.dx + r0 * c.D;
-				d.splits = std::min(l.splits, split16::choose_splits(n, c.D, c.V));
-				d.C = d.splits > 1 ? m.at<float>(l.slabs) : out;
-				d.ldc = c.D; d.slab = d.splits > 1 ? n * c.D : 0;
-				NNB_TRY(split16::run(s, d, split16::kStore, parts, G, false, W, true, n, c.D, c.V));
-				if (d.splits > 1) NNB_TRY(split16::sum_slabs(s, d.C, d.splits, n * c.D, out, 0));
-			}
-			if (c.dw) {                                    // dW (+)= G^T X
-				split16::Product d;
-				d.rb = xr; d.shift = kGShift;
-				d.C = c.dw + z * c.dw_stride; d.ldc = c.D; d.accumulate = !first;
-				NNB_TRY(split16::run(s, d, split16::kStore, parts, G, true, X, true, c.V, c.D, n));
-			}
+				d.rb = rb; d.shift = kGShift;
+				d.splits = split16::split_count(K, std::min(max_splits, split16::choose_splits(M, c.D, K)));
+				const bool cut = d.splits > 1;
+				d.C = cut ? m.at<float>(l.slabs) : out;
+				d.ldc = c.D; d.slab = cut ? M * c.D : 0;
+				d.accumulate = !cut && accumulate;
+				NNB_TRY(split16::run(s, d, split16::kStore, parts, a, mn_a, b, true, M, c.D, K));
+				return cut ? split16::sum_slabs(s, d.C, d.splits, M * c.D, out, accumulate) : NNB_OK;
+			};
+			if (c.dx) NNB_TRY(product(G, false, W, wr, n, c.V, l.dx_splits, c.dx + r0 * c.D, 0));                        // G W
+			if (c.dw) NNB_TRY(product(G, true, X, xr, c.V, n, l.dw_splits, c.dw + z * c.dw_stride, !first));             // G^T X
 			r0 += n;
 		}
 	}

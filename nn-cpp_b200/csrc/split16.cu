@@ -511,13 +511,32 @@ nnb_status pack(cudaStream_t s, const float* x, long long rows, long long cols, 
 	return cuda_status(cudaGetLastError(), "split pack launch");
 }
 
-int choose_splits(long long M, long long N, long long K) {
-	// A product with fewer tiles than SMs is cut along its depth until two waves of items are there, in
-	// pieces of whole chunks and at least 1024 terms
-	const long long tiles = (M + kBM - 1) / kBM * ((N + kBN - 1) / kBN), chunks = (K + kBK * kChunkKb - 1) / (kBK * kChunkKb);
-	if (tiles >= 148) return 1;
-	const long long want = std::max<long long>(1, std::min<long long>(2 * 148 / tiles, chunks / 8)), per = (chunks + want - 1) / want;
+// Chunks of 128 terms in a depth of K.
+static long long chunks_of(long long K) { return (K + kBK * kChunkKb - 1) / (kBK * kChunkKb); }
+
+int split_count(long long K, int want) {
+	const long long chunks = chunks_of(K), per = (chunks + want - 1) / want;
 	return (int)((chunks + per - 1) / per);
+}
+
+int choose_splits(long long M, long long N, long long K) {
+	// Items are worked through in waves of one per SM, so n pieces of the depth take
+	// ceil(tiles n / 148) / n of a tile's time, K times 21 ns (3.1 TFLOP/s per SM); writing and reading back the
+	// slabs adds tiles n times 44 ns (256 KB each at 6 TB/s). The fewest pieces of about the least cost, each of
+	// at least 512 terms.
+	const long long tiles = (M + kBM - 1) / kBM * ((N + kBN - 1) / kBN), chunks = chunks_of(K);
+	int best = 1;
+	double best_cost = 0.0;
+	for (int want = 1; want <= (int)std::min<long long>(16, std::max<long long>(1, chunks / 4)); ++want) {
+		const int n = split_count(K, want);
+		const double waves = (double)((tiles * n + 147) / 148) * ((chunks + n - 1) / n) / chunks;
+		const double cost = waves + (n > 1 ? 44.0 / 21.0 * n * tiles / K : 0.0);
+		if (n == 1 || cost < 0.95 * best_cost) {
+			best = n;
+			best_cost = cost;
+		}
+	}
+	return best;
 }
 
 nnb_status run(cudaStream_t s, Product p, int epilogue, int parts, const Pack& a, bool mn_a, const Pack& b, bool mn_b,
