@@ -301,17 +301,18 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 		const int row = quad * 32 + lane;
 		float* stage = reinterpret_cast<float*>(smem + (size_t)kStages * kStageBytes + (warp - 4) * kEpiTile);
 		float4* st4 = reinterpret_cast<float4*>(stage);
-		float alpha_a = exp2_int(-p.shift), alpha_b = 1.0f;
-		if (p.ra) alpha_a *= exp2_int(-range_shift(p.ra));
-		if (p.rb) alpha_b = exp2_int(-range_shift(p.rb));
+		// acc is scaled back by 2^e: in one factor, or two where the exponent does not fit one
+		const int e = -p.shift - (p.ra ? range_shift(p.ra) : 0) - (p.rb ? range_shift(p.rb) : 0);
+		const int e1 = max(-126, min(127, e)), e2 = max(-126, min(127, e - e1));
+		const float alpha = exp2_int(e1), alpha2 = exp2_int(e2);
 		const bool vec_ok = kEpi == kStore && p.ldc % 4 == 0 && p.slab % 4 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15) == 0;
 		int v = 0;
 		bool ok = true;
 		for (int t = blockIdx.x; ok && t < items; t += gridDim.x) {
 			const Item it = item_at(t, p);
-			float acc[kBN / 2];
+			float2 acc[kBN / 4];                           // this thread's row, 128 columns in pairs
 #pragma unroll
-			for (int j = 0; j < kBN / 2; ++j) acc[j] = 0.0f;
+			for (int j = 0; j < kBN / 4; ++j) acc[j] = make_float2(0.0f, 0.0f);
 			for (int c0 = it.kb0; c0 < it.kb1; c0 += kChunkKb, ++v) {
 				if (!mbar_wait_warp(smem_u32(&accf_bar[v & 1]), (v >> 1) & 1, p.err, kDevTimeoutAccum, abort_flag)) {
 					ok = false;
@@ -320,12 +321,13 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 				tc_fence_after();
 				const uint32_t src = tmem_base + ((uint32_t)(quad * 32) << 16) + (v & 1) * kBN + half * (kBN / 2);
 #pragma unroll
-				for (int c = 0; c < kBN / 32; ++c) {
-					uint32_t r[16];
-					tmem_ld_32x32b_x16(src + c * 16, r);
+				for (int c = 0; c < kBN / 64; ++c) {
+					uint32_t r[32];
+					tmem_ld_32x32b_x32(src + c * 32, r);
 					tmem_wait_ld();
 #pragma unroll
-					for (int j = 0; j < 16; ++j) acc[c * 16 + j] += __uint_as_float(r[j]);
+					for (int j = 0; j < 16; ++j)
+						acc[c * 16 + j] = add2_rn(acc[c * 16 + j], make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
 				}
 				tc_fence_before();
 				__syncwarp();
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 #pragma unroll
 				for (int g = 0; g < 8; ++g)
 					st4[lane * 8 + (g ^ (lane & 7))] =
-						make_float4(acc[c * 32 + 4 * g], acc[c * 32 + 4 * g + 1], acc[c * 32 + 4 * g + 2], acc[c * 32 + 4 * g + 3]);
+						make_float4(acc[c * 16 + 2 * g].x, acc[c * 16 + 2 * g].y, acc[c * 16 + 2 * g + 1].x, acc[c * 16 + 2 * g + 1].y);
 				__syncwarp();
 				const int g = lane & 7;
 #pragma unroll
@@ -357,48 +359,96 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 				}
 				__syncwarp();
 			};
+			if (alpha2 != 1.0f) {
+#pragma unroll
+				for (int j = 0; j < kBN / 4; ++j) acc[j] = mul2_rn(acc[j], make_float2(alpha2, alpha2));
+			}
 			const int warp_row = it.mt * kBM + quad * 32, rows_here = max(0, min(32, p.M - warp_row));
 			if (kEpi == kStore) {
 				float* C = p.C + it.split * p.slab;
 #pragma unroll
+				for (int j = 0; j < kBN / 4; ++j) acc[j] = mul2_rn(acc[j], make_float2(alpha, alpha));
+#pragma unroll
 				for (int c = 0; c < kBN / 64; ++c) {
 					const int gn = n0 + c * 32;
 					if (gn >= p.N) break;                  // warp-uniform
-#pragma unroll
-					for (int j = 0; j < 32; ++j) acc[c * 32 + j] = acc[c * 32 + j] * alpha_a * alpha_b;
 					if (vec_ok && gn + 32 <= p.N) {
 						stage_rows(C + (long long)warp_row * p.ldc + gn, p.ldc, rows_here, c, p.accumulate != 0);
 					} else if (gm < p.M) {
 						float* dst = C + (long long)gm * p.ldc + gn;
 #pragma unroll
-						for (int j = 0; j < 32; ++j)
-							if (gn + j < p.N) dst[j] = p.accumulate ? dst[j] + acc[c * 32 + j] : acc[c * 32 + j];
+						for (int j = 0; j < 32; ++j) {
+							const float a = j & 1 ? acc[c * 16 + j / 2].y : acc[c * 16 + j / 2].x;
+							if (gn + j < p.N) dst[j] = p.accumulate ? dst[j] + a : a;
+						}
 					}
 				}
 			} else {
+				// l = acc 2^e + bias: the biases of the warp's 128 columns through its staging tile (one coalesced
+				// load, then broadcasts)
+				if (p.bias) {
+					float4 b;
+					b.x = n0 + 4 * lane < p.N ? __ldg(p.bias + n0 + 4 * lane) : 0.0f;
+					b.y = n0 + 4 * lane + 1 < p.N ? __ldg(p.bias + n0 + 4 * lane + 1) : 0.0f;
+					b.z = n0 + 4 * lane + 2 < p.N ? __ldg(p.bias + n0 + 4 * lane + 2) : 0.0f;
+					b.w = n0 + 4 * lane + 3 < p.N ? __ldg(p.bias + n0 + 4 * lane + 3) : 0.0f;
+					st4[lane] = b;
+					__syncwarp();
+#pragma unroll
+					for (int j = 0; j < kBN / 8; ++j) {
+						const float4 bj = st4[j];
+						acc[2 * j] = fma2_rn(acc[2 * j], make_float2(alpha, alpha), make_float2(bj.x, bj.y));
+						acc[2 * j + 1] = fma2_rn(acc[2 * j + 1], make_float2(alpha, alpha), make_float2(bj.z, bj.w));
+					}
+					__syncwarp();                          // read before the tile is written again
+				} else {
+#pragma unroll
+					for (int j = 0; j < kBN / 4; ++j) acc[j] = mul2_rn(acc[j], make_float2(alpha, alpha));
+				}
+				const long long slot = (long long)(it.nt * 2 + half) * (p.tiles_m * kBM) + gm;
+				if (p.part_sum) {
+					float total = 0.0f;
+#pragma unroll
+					for (int j = 0; j < kBN / 4; ++j) {
+						if (n0 + 2 * j < p.N) total += acc[j].x;
+						if (n0 + 2 * j + 1 < p.N) total += acc[j].y;
+					}
+					p.part_sum[slot] = total;
+				}
 				const int64_t target = gm < p.M ? p.targets[gm] : -1;
 				const int tj = target >= n0 && target < n0 + kBN / 2 && target < p.N ? (int)(target - n0) : -1;
-				float top = -INFINITY, total = 0.0f, at = 0.0f;
+				if (__any_sync(0xffffffffu, tj >= 0)) {
+					float at = 0.0f;
 #pragma unroll
-				for (int j = 0; j < kBN / 2; ++j) {
-					const bool in = n0 + j < p.N;          // warp-uniform
-					const float l = acc[j] * alpha_a * alpha_b + (in && p.bias ? __ldg(p.bias + n0 + j) : 0.0f);
-					acc[j] = l;
-					if (in) {
-						top = fmaxf(top, l);
-						total += l;
+					for (int j = 0; j < kBN / 4; ++j) {
+						if (tj == 2 * j) at = acc[j].x;
+						if (tj == 2 * j + 1) at = acc[j].y;
 					}
-					if (j == tj) at = l;
+					if (tj >= 0) p.target_logit[gm] = at;
 				}
-				float sum = 0.0f;
+				if (n0 + kBN / 2 > p.N) {                      // columns past N: no part of the softmax
 #pragma unroll
-				for (int j = 0; j < kBN / 2; ++j)
-					if (n0 + j < p.N) sum += exp2_hw((acc[j] - top) * kLog2e);
-				if (top == -INFINITY && sum != sum) sum = total != total ? total : 0.0f;   // all -inf: an empty part
-				const long long slot = (long long)(it.nt * 2 + half) * (p.tiles_m * kBM) + gm;
-				p.part[slot] = make_float2(top, sum);
-				if (p.part_sum) p.part_sum[slot] = total;
-				if (tj >= 0) p.target_logit[gm] = at;
+					for (int j = 0; j < kBN / 4; ++j) {
+						if (n0 + 2 * j >= p.N) acc[j].x = -INFINITY;
+						if (n0 + 2 * j + 1 >= p.N) acc[j].y = -INFINITY;
+					}
+				}
+				float2 top2 = make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+				for (int j = 0; j < kBN / 4; ++j) {
+					top2.x = fmaxf(top2.x, acc[j].x);
+					top2.y = fmaxf(top2.y, acc[j].y);
+				}
+				const float top = fmaxf(top2.x, top2.y);
+				// all -inf: an empty part (top stands in as 0, every term is 0); NaN and +inf give a NaN sum
+				const float base = top == -INFINITY ? 0.0f : top;
+				float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+				for (int j = 0; j < kBN / 4; ++j) {
+					const float2 a = mul2_rn(add2_rn(acc[j], make_float2(-base, -base)), make_float2(kLog2e, kLog2e));
+					sum = add2_rn(sum, make_float2(exp2_hw(a.x), exp2_hw(a.y)));
+				}
+				p.part[slot] = make_float2(top, sum.x + sum.y);
 				if (kEpi == kLogits) {
 #pragma unroll
 					for (int c = 0; c < kBN / 64; ++c) {
