@@ -231,7 +231,7 @@ NNB_API nnb_status nnb_layernorm_bwd_grouped(void* stream, size_t R, size_t D, s
  *   p = branch, or norm(branch; post_gamma, post_beta) when post_gamma is not NULL
  *   h = x + scale * gate * p          gate NULL: 1
  *   y = norm(h; gamma, beta)
- * over R rows of D values (D <= 16384). kind NNB_NORM_LAYER: (a - mean) / sqrt(var + eps) * gamma + beta;
+ * over R rows of D values (D <= 16384). branch and h NULL: y = norm(x) alone. kind NNB_NORM_LAYER: (a - mean) / sqrt(var + eps) * gamma + beta;
  * NNB_NORM_RMS: a / sqrt(mean a^2 + eps) * gamma, beta and post_beta NULL. gate holds gate_rows rows of D,
  * each serving R / gate_rows consecutive rows (1: a parameter per channel; ignored when gate is NULL).
  * stats (R rows of 4 floats, 16-byte aligned; NULL: not kept) is what the backward needs. No other buffer
@@ -248,7 +248,8 @@ typedef struct nnb_grad_out {
 	int first;
 } nnb_grad_out;
 /* Gradients of nnb_residual_norm_fwd from dh and dy (either may be NULL: zeros), the forward's h and
- * stats, and its operands (branch may be NULL without post_gamma and gate). Each nnb_grad_out may be
+ * stats, and its operands (branch may be NULL without post_gamma and gate; after a forward without a
+ * branch h is x). Each nnb_grad_out may be
  * NULL. dx also receives what reaches h through y. Parameter gradients (a gate of one row included) are
  * kept per group of R / groups consecutive rows, as nnb_layernorm_bwd_grouped's; a gate of several rows
  * needs gate_rows % groups == 0. The sums' order depends on D, R / groups and the gate's span only. */

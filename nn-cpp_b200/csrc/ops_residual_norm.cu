@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta) residual_norm_fwd_kernel(
 	for (int u = 0; u < KV; ++u) {
 		in[u] = j0 + u * T * VEC < p.D;
 		a[u].zero();
-		if (in[u]) a[u].load(p.branch + off + u * T * VEC);
+		if (in[u] && p.branch) a[u].load(p.branch + off + u * T * VEC);
 	}
 #pragma unroll
 	for (int u = 0; u < KV; ++u) {
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta) residual_norm_fwd_kernel(
 	for (int u = 0; u < KV; ++u) {
 #pragma unroll
 		for (int i = 0; i < VEC; ++i) a[u].v[i] = __fmaf_rn(p.scale, a[u].v[i], xv[u].v[i]);
-		if (in[u]) a[u].store(p.h + off + u * T * VEC);
+		if (in[u] && p.h) a[u].store(p.h + off + u * T * VEC);
 	}
 	const float2 sh = row_stats<VEC, KV, T>(a, in, p.layer, inv_d, p.eps, sum);
 	affine<VEC, KV, T>(a, in, sh, p.gamma + j0, p.beta ? p.beta + j0 : nullptr);
@@ -270,7 +270,8 @@ nnb_status nnb_residual_norm_fwd(void* stream, size_t R, size_t D, size_t gate_r
 	NNB_TRY(check_common("residual_norm_fwd", R, D, gate_rows, kind, gate, post_gamma != nullptr, post_beta, gamma, beta,
 		true));
 	if (R == 0) return NNB_OK;
-	if (!x || !branch || !h || !y) return fail(NNB_ERR_INVALID, "residual_norm_fwd: null pointer");
+	if (!x || !y || (!branch) != (!h)) return fail(NNB_ERR_INVALID, "residual_norm_fwd: null pointer");
+	if (!branch && (gate || post_gamma)) return fail(NNB_ERR_INVALID, "residual_norm_fwd: a gate or post_gamma without a branch");
 	if (reinterpret_cast<uintptr_t>(stats) & 15) return fail(NNB_ERR_INVALID, "residual_norm_fwd: stats must be 16-byte aligned");
 	Row p;
 	p.x = x; p.branch = branch; p.post_gamma = post_gamma; p.post_beta = post_beta; p.gate = gate;

@@ -431,6 +431,29 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     return h, Value.node(y_data, (h,) + norm_parents, y_backward)
 
 
+def rmsnorm(x: Value, gamma: Value, eps: float) -> Value:
+    """x / sqrt(mean(x^2) + eps) * gamma over the last axis (residual_norm's "rms" norm on its own)."""
+    if not x.shape or 0 in x.shape or gamma.shape != (x.shape[-1],):
+        raise TensorShapeError("rmsnorm: shapes do not agree")
+    _check_buffers("rmsnorm", (x, gamma))
+    D = x.shape[-1]
+    R = x.data.numel() // D
+    if R % _GROUPS:
+        raise TensorShapeError("rmsnorm: the rows do not divide into the parameter groups")
+    y, stats = empty(x.shape), empty((R, 4))
+    check(lib().nnb_residual_norm_fwd(_s(), R, D, 0, NORM_RMS, eps, 1.0, _p(x.data), None, None, None, None, _p(gamma.data),
+                                      None, None, _p(y), _p(stats)))
+
+    def backward(g):
+        dx, fx = x.grad_accum() if _need(x) else (None, 0)
+        dg, fg = gamma.grad_accum() if _need(gamma) else (None, 0)
+        check(lib().nnb_residual_norm_bwd(_s(), R, D, _GROUPS, 0, NORM_RMS, 1.0, None, _p(g), _p(x.data), None, None, None,
+                                          None, _p(gamma.data), _p(stats), ctypes.byref(GradOut(_p(dx), 0, fx)), None, None,
+                                          None, None, ctypes.byref(GradOut(_p(dg), _gstride(dg, gamma), fg)), None))
+
+    return Value.node(y, (x, gamma), backward)
+
+
 def batchnorm(x: Value, weight: Value, bias: Value, eps: float, fuse_relu: bool = False,
               mean_out: torch.Tensor | None = None, var_out: torch.Tensor | None = None) -> Value:
     """batchnorm in training mode (ops.cpp:900-1001); mean_out / var_out receive the batch statistics

@@ -110,6 +110,22 @@ class LayerNorm(Module):
         return [("gamma", self.gamma), ("beta", self.beta)]
 
 
+class RMSNorm(Module):
+    """x / sqrt(mean(x^2) + eps) * gamma (no reference counterpart: nn-cpp has LayerNorm only)."""
+
+    beta = None
+
+    def __init__(self, dim: int, device, eps: float = 1e-5):
+        self.eps = eps
+        self.gamma = _param(np.ones(dim), device)
+
+    def forward(self, x: Value) -> Value:
+        return F.rmsnorm(x, self.gamma, self.eps)
+
+    def named_parameters(self):
+        return [("gamma", self.gamma)]
+
+
 class Embedding(Module):
     def __init__(self, num: int, dim: int, rng: np.random.Generator, device):
         lim = 1.0 / math.sqrt(dim)
@@ -203,26 +219,70 @@ class MultiHeadAttention(Module):
 class TransformerBlock(Module):
     """x + attn(ln1(x)), then + drop(fc2(gelu(fc1(ln2(.))))) (transformer.cpp:41-44); fc1 + gelu run as
     one GEMM with the GELU in its epilogue. The attention's and the block's Dropout layers are built
-    in the reference's member order (attention first), so their streams match its own."""
+    in the reference's member order (attention first), so their streams match its own.
 
-    def __init__(self, dim: int, heads: int, mlp_ratio: int, causal: bool, rng, device, dropout: float = 0.0):
-        self.ln1 = LayerNorm(dim, device)
+    residual (a ResidualConfig) selects the forms the reference does not have: RMS norms, a norm on each
+    branch (post1., post2.), a learned gate per channel (scale1, scale2) and a scale on the residual sums.
+    Such a block runs every residual sum joined with the norm after it (F.residual_norm), see advance."""
+
+    def __init__(self, dim: int, heads: int, mlp_ratio: int, causal: bool, rng, device, dropout: float = 0.0,
+                 residual: "ResidualConfig | None" = None):
+        self.residual = residual
+        norm = residual.norm_class() if residual else LayerNorm
+        self.ln1 = norm(dim, device)
         self.attn = MultiHeadAttention(dim, heads, causal, rng, device, dropout)
-        self.ln2 = LayerNorm(dim, device)
+        self.ln2 = norm(dim, device)
         self.fc1 = Linear(dim, mlp_ratio * dim, rng, device)
         self.fc2 = Linear(mlp_ratio * dim, dim, rng, device)
         self.drop = Dropout(dropout, device)
+        self.post1 = self.post2 = self.scale1 = self.scale2 = None
+        if residual and residual.post_norm:
+            self.post1, self.post2 = norm(dim, device), norm(dim, device)
+        if residual and residual.layer_scale is not None:
+            self.scale1, self.scale2 = (_param(np.full(dim, residual.layer_scale), device) for _ in range(2))
+
+    def _mlp(self, y: Value) -> Value:
+        return self.drop(self.fc2(F.linear_gelu(y, self.fc1.weight, self.fc1.bias)))
 
     def forward(self, x: Value) -> Value:
+        if self.residual:                # the norm after the last sum is the caller's; ln1 stands in for it
+            return self.advance(x, self.ln1(x), self.ln1)[0]
         h = F.add(x, self.attn(self.ln1(x)))
-        return F.add(h, self.drop(self.fc2(F.linear_gelu(self.ln2(h), self.fc1.weight, self.fc1.bias))))
+        return F.add(h, self._mlp(self.ln2(h)))
+
+    def _join(self, x: Value, branch: Value, norm, post, gate) -> tuple[Value, Value]:
+        r = self.residual
+        return F.residual_norm(x, branch, norm.gamma, norm.beta, norm.eps, kind=r.norm, gate=gate, scale=r.residual_scale,
+                               post_gamma=post.gamma if post else None, post_beta=post.beta if post else None)
+
+    def advance(self, x: Value, y: Value, next_norm) -> tuple[Value, Value]:
+        """The block as a step of a chain of residual blocks: from the stream x and y = ln1(x) to the new
+        stream and next_norm of it (the next block's ln1, or the model's last norm)."""
+        h, y = self._join(x, self.attn(y), self.ln2, self.post1, self.scale1)
+        return self._join(h, self._mlp(y), next_norm, self.post2, self.scale2)
 
     def named_parameters(self):
         out = []
         for name, m in (("ln1.", self.ln1), ("attn.", self.attn), ("ln2.", self.ln2), ("fc1.", self.fc1),
-                        ("fc2.", self.fc2)):
-            out += [(name + n, p) for n, p in m.named_parameters()]
-        return out
+                        ("fc2.", self.fc2), ("post1.", self.post1), ("post2.", self.post2)):
+            out += [(name + n, p) for n, p in m.named_parameters()] if m else []
+        return out + [(n, p) for n, p in (("scale1", self.scale1), ("scale2", self.scale2)) if p]
+
+
+@dataclass
+class ResidualConfig:
+    """A residual stream's norms and gates (no reference counterpart; F.residual_norm): norm "layer" or
+    "rms"; post_norm puts one on every branch before its sum; layer_scale starts a learned gate per channel
+    on every branch at that value; residual_scale multiplies every branch."""
+    norm: str = "layer"
+    post_norm: bool = False
+    layer_scale: float | None = None
+    residual_scale: float = 1.0
+
+    def norm_class(self):
+        if self.norm not in ("layer", "rms"):
+            raise ValueError('ResidualConfig: norm must be "layer" or "rms"')
+        return LayerNorm if self.norm == "layer" else RMSNorm
 
 
 @dataclass
@@ -236,6 +296,7 @@ class TransformerConfig:
     mlp_ratio: int = 4
     dropout: float = 0.0
     causal: bool = True
+    residual: ResidualConfig | None = None
 
 
 class Transformer(Module):
@@ -249,16 +310,31 @@ class Transformer(Module):
         self.config = c
         self.embed = Embedding(c.vocab_size, c.dim, rng, device)
         self.pos = PositionalEncoding(c.max_len, c.dim, device)
-        self.blocks = [TransformerBlock(c.dim, c.heads, c.mlp_ratio, c.causal, rng, device, c.dropout)
+        self.blocks = [TransformerBlock(c.dim, c.heads, c.mlp_ratio, c.causal, rng, device, c.dropout, c.residual)
                        for _ in range(c.layers)]
-        self.ln_f = LayerNorm(c.dim, device)
+        self.ln_f = (c.residual.norm_class() if c.residual else LayerNorm)(c.dim, device)
         self.head = Linear(c.dim, c.vocab_size, rng, device)
 
-    def forward(self, ids: torch.Tensor) -> Value:
+    def features(self, ids: torch.Tensor) -> Value:
+        """The normed residual stream that the head reads."""
         h = self.pos(self.embed(ids))
+        if self.config.residual:
+            y = self.blocks[0].ln1(h)
+            for b, following in zip(self.blocks, [b.ln1 for b in self.blocks[1:]] + [self.ln_f]):
+                h, y = b.advance(h, y, following)
+            return y
         for b in self.blocks:
             h = b(h)
-        return self.head(self.ln_f(h))
+        return self.ln_f(h)
+
+    def forward(self, ids: torch.Tensor) -> Value:
+        return self.head(self.features(ids))
+
+    def loss(self, ids: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, label_smoothing: float = 0.0,
+             grad_norm: torch.Tensor | None = None) -> Value:
+        """sequence_cross_entropy of forward(ids) without keeping the logits (F.linear_cross_entropy)."""
+        return F.linear_cross_entropy(self.features(ids), self.head.weight, self.head.bias, targets, ignore_index,
+                                      label_smoothing, grad_norm)
 
     def named_parameters(self):
         out = [("embed." + n, p) for n, p in self.embed.named_parameters()]

@@ -71,12 +71,17 @@ def gather_weight_slices(flat_w: torch.Tensor, chunk: int, rank: int, group=None
 
 
 class ShardedTrainer:
-    def __init__(self, model, optimizer, shards: int = 8, world: int = 1, rank: int = 0, group=None):
+    """fused_loss: the loss through the model's own loss method (nnb.nn.Transformer.loss, which keeps no
+    logits) instead of sequence_cross_entropy of its forward; the step is as independent of the number of
+    GPUs, its bits differ from the other loss's."""
+
+    def __init__(self, model, optimizer, shards: int = 8, world: int = 1, rank: int = 0, group=None,
+                 fused_loss: bool = False):
         if shards % world:
             raise ValueError("the virtual shard count must be a multiple of the number of ranks")
         if getattr(optimizer, "state_bits", 32) != 32:
             raise ValueError("ShardedTrainer keeps 32-bit moments of its own: use an AdamW with state_bits=32")
-        self.model, self.opt = model, optimizer
+        self.model, self.opt, self.fused_loss = model, optimizer, fused_loss
         self.shards, self.world, self.rank, self.group = shards, world, rank, group
         self.owned = shard_owners(shards, world, rank)
         self.params = model.parameters()
@@ -197,8 +202,11 @@ class ShardedTrainer:
         groups = len(self.owned)
         # with several ranks each dropout mask is this rank's rows of the whole batch's draw
         with F.param_groups(groups), F.batch_slice(B, lo, hi):
-            logits = self.model(ids[lo:hi])
-            loss = F.sequence_cross_entropy(logits, targets[lo:hi], grad_norm=self.grad_norm)
+            if self.fused_loss:
+                loss = self.model.loss(ids[lo:hi], targets[lo:hi].contiguous(), grad_norm=self.grad_norm)
+            else:
+                logits = self.model(ids[lo:hi])
+                loss = F.sequence_cross_entropy(logits, targets[lo:hi], grad_norm=self.grad_norm)
             loss.backward()
         if any(p.grad_fresh for p in self.params):
             raise RuntimeError("a parameter received no gradient")

@@ -32,8 +32,9 @@ def test_forward_refusals():
     assert _fwd(D=0) == SHAPE
     assert _fwd(D=16385) == UNSUP and "16384" in nnb.last_error()
     assert _fwd(R=2 ** 41) == UNSUP
-    for name in ("x", "branch", "gamma", "beta", "h", "y"):
+    for name in ("x", "branch", "gamma", "beta", "h", "y"):        # (branch and h go together)
         assert _fwd(**{name: None}) == INV, name
+    assert _fwd(branch=None, h=None, gate=P, gate_rows=1) == INV and _fwd(branch=None, h=None, pg=P, pb=P) == INV
     assert _fwd(kind=NORM_RMS) == INV                                  # an rms norm with a beta
     assert _fwd(pg=P) == INV and _fwd(pb=P) == INV                     # half a layer norm after the block
     assert _fwd(kind=NORM_RMS, beta=None, pg=P, pb=P) == INV
@@ -82,6 +83,15 @@ def test_function_refusals():
             F.residual_norm(*args, **kw)
     with pytest.raises(ValueError, match="current CUDA device"):
         F.residual_norm(x, b, g, be)
+
+
+def test_rmsnorm_refusals():
+    x, g = _values((3, 8), (8,))
+    for args in ((x, _values((7,))[0], 1e-5), (_values((0, 8))[0], g, 1e-5)):
+        with pytest.raises(TensorShapeError):
+            F.rmsnorm(*args)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        F.rmsnorm(x, g, 1e-5)
 
 
 def test_backward_from_several_roots_refusals():

@@ -316,6 +316,21 @@ def test_captured_and_on_another_stream(cuda):
         assert all(torch.equal(res[2][k], want[2][k]) for k in want[2])
 
 
+@pytest.mark.parametrize("R,D", [(1, 16), (50, 33), (300, 512), (7, 4100)])
+def test_rmsnorm(cuda, R, D):
+    ops, _, dy = _make(R, D, 1, "rms", False, "none", seed=15)
+    x, gamma = Value.leaf(ops["x"], True), Value.leaf(ops["gamma"], True)
+    y = F.rmsnorm(x, gamma, EPS)
+    y.backward(dy)
+    norm = Norm64(ops["x"].double(), ops["gamma"].double(), None, False)
+    assert torch.all((y.data.double() - norm.out).abs() <= norm.err_out)
+    want, err = norm.back(dy.double(), torch.zeros_like(norm.hat))
+    assert torch.all((x.grad.double() - want).abs() <= err + E * want.abs())
+    terms = dy.double() * norm.hat
+    err = (dy.double().abs() * norm.err_hat).sum(0) + (R + 60) * E * terms.abs().sum(0)
+    assert torch.all((gamma.grad.double() - terms.sum(0)).abs() <= err)
+
+
 def test_no_rows(cuda):
     """The C entry with R == 0: stored parameter gradients become zeros, added ones stay."""
     import ctypes
