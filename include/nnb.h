@@ -427,10 +427,17 @@ NNB_API nnb_status nnb_sequence_ce_bwd(void* stream, size_t P, size_t V, const f
 NNB_API nnb_status nnb_linear_ce_fwd(void* stream, size_t P, size_t D, size_t V, size_t groups, const float* x,
 		const float* w, const float* bias, const int64_t* targets, int64_t ignore_index, float label_smoothing,
 		float* row_loss, float* loss, float* norm, float* dx, float* dw, size_t dw_stride, float* db, size_t db_stride);
-/* dst_z (+)= src_z * (a * b) for `groups` runs of n values, src back to back, dst dst_stride apart (0: back
- * to back); a and b are device scalars. */
-NNB_API nnb_status nnb_scaled_accumulate(void* stream, size_t groups, size_t n, const float* src, const float* a,
-		const float* b, float* dst, size_t dst_stride, int first);
+/* dst_z (+)= src_z * (a * b) for `groups` runs of n values per entry, src back to back, dst dst_stride apart (0:
+ * back to back), stored when first != 0; a and b are device scalars. At most 8 entries (a host array, read
+ * before the call returns; their buffers must not overlap), one launch. */
+typedef struct nnb_scaled_grad {
+	const float* src;
+	float* dst;
+	size_t n, groups, dst_stride;
+	int first;
+} nnb_scaled_grad;
+NNB_API nnb_status nnb_scaled_accumulate(void* stream, size_t count, const nnb_scaled_grad* grads, const float* a,
+		const float* b);
 /* embedding (ops.cpp:1991-2015): out[i] = weight[ids[i]]; the backward adds g rows into dweight in
  * token order per row (deterministic, no float atomics), starting from 0 when first != 0 and from
  * dweight's contents otherwise; V <= 40000 for the backward. */

@@ -90,12 +90,20 @@ struct Product {
 	int* err = nullptr;
 };
 
-// Range of x[rows x cols] (leading dimension cols) into *out (zeroed here).
-nnb_status find_range(cudaStream_t s, const float* x, long long n, Range* out);
-// Packs x [rows x cols] (row-major, dense) into buf, rows padded with zeros to `row_blocks` blocks; values that
-// are not finite become zero and set row_bad[row] (nullable, zeroed by the caller).
-nnb_status pack(cudaStream_t s, const float* x, long long rows, long long cols, long long row_blocks, int parts,
-		const Range* range, void* buf, int* row_bad);
+// Ranges of x0[n0] and x1[n1] into out[0] and out[1], which the caller has zeroed.
+nnb_status find_ranges(cudaStream_t s, const float* x0, long long n0, const float* x1, long long n1, Range* out);
+
+// A matrix to pack: x [rows x cols] (row-major, dense) into buf, rows padded with zeros to `row_blocks` blocks;
+// values that are not finite become zero and set row_bad[row] (nullable, zeroed by the caller).
+struct PackJob {
+	const float* x;
+	long long rows, cols, row_blocks;
+	const Range* range;
+	void* buf;
+	int* row_bad;
+};
+// One or two of them in one launch.
+nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts);
 
 // C = A B^T with A = a (K-major: rows of a) or a^T (mn_a: columns of a), B likewise; p's sizes, operands'
 // widths and tile counts are filled in here. parts: 2 or 1.

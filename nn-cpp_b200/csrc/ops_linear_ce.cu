@@ -221,25 +221,33 @@ __global__ void __launch_bounds__(1024) ce_mean_kernel(long long rows, const flo
 	}
 }
 
-// dst[z] (+)= src[z] * (a b) for `groups` runs of n values, dst's dst_stride apart.
-__global__ void scaled_accumulate_kernel(long long n, const float* __restrict__ src, const float* __restrict__ a,
-		const float* __restrict__ b, float* __restrict__ dst, long long dst_stride, int first, int vec) {
-	const float k = *a * *b;
-	src += blockIdx.y * n;
-	dst += blockIdx.y * dst_stride;
-	const long long step = (long long)gridDim.x * blockDim.x;
-	long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-	if (vec) {
-		const float4* s4 = reinterpret_cast<const float4*>(src);
-		float4* d4 = reinterpret_cast<float4*>(dst);
-		for (; i < n / 4; i += step) {
-			const float4 v = __ldg(s4 + i);
-			float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-			if (!first) o = d4[i];
-			d4[i] = make_float4(o.x + v.x * k, o.y + v.y * k, o.z + v.z * k, o.w + v.w * k);
+constexpr int kScaledMax = 8;
+struct ScaledList {
+	nnb_scaled_grad g[kScaledMax];
+	int vec[kScaledMax];
+	const float *a, *b;
+};
+
+// dst_z (+)= src_z (a b) for the groups z of every entry (grid.y).
+__global__ void __launch_bounds__(256) scaled_accumulate_kernel(const ScaledList l) {
+	const nnb_scaled_grad& e = l.g[blockIdx.y];
+	const float k = *l.a * *l.b;
+	const long long n = (long long)e.n, step = gridDim.x * 256LL, i0 = blockIdx.x * 256LL + threadIdx.x;
+	for (size_t z = 0; z < e.groups; ++z) {
+		const float* __restrict__ src = e.src + z * e.n;
+		float* __restrict__ dst = e.dst + z * e.dst_stride;
+		if (l.vec[blockIdx.y]) {
+			const float4* s4 = reinterpret_cast<const float4*>(src);
+			float4* d4 = reinterpret_cast<float4*>(dst);
+			for (long long i = i0; i < n / 4; i += step) {
+				const float4 v = __ldg(s4 + i);
+				float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+				if (!e.first) o = d4[i];
+				d4[i] = make_float4(o.x + v.x * k, o.y + v.y * k, o.z + v.z * k, o.w + v.w * k);
+			}
+		} else {
+			for (long long i = i0; i < n; i += step) dst[i] = (e.first ? 0.0f : dst[i]) + __ldg(src + i) * k;
 		}
-	} else {
-		for (; i < n; i += step) dst[i] = (first ? 0.0f : dst[i]) + __ldg(src + i) * k;
 	}
 }
 
@@ -289,10 +297,10 @@ Layout plan(const Call& c, Scratch& s) {
 	const size_t pad = (size_t)l.blocks * kRows;
 	l.dx_splits = c.dx ? split16::choose_splits(l.piece, c.D, c.V) : 1;
 	l.dw_splits = c.dw ? split16::choose_splits(c.V, c.D, l.piece) : 1;
-	l.ranges = s.take(2 * sizeof(split16::Range));
+	l.ranges = s.take(2 * sizeof(split16::Range) + (size_t)c.P * sizeof(int));      // and x_bad: zeroed together
+	l.x_bad = l.ranges + 2 * sizeof(split16::Range);
 	l.wpack = s.take(split16::pack_bytes(c.V, c.D));
 	l.xpack = s.take(split16::pack_bytes(l.piece, c.D));
-	l.x_bad = s.take(pad * sizeof(int));
 	l.g = s.take(c.grad() ? (size_t)l.blocks * c.kw() * kBlockBytes : 0);
 	l.part = s.take((size_t)c.parts() * pad * sizeof(float2));
 	l.part_sum = s.take(c.ls != 0.0f ? (size_t)c.parts() * pad * sizeof(float) : 0);
@@ -312,9 +320,8 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 	split16::Range* wr = xr + 1;
 	float* row_loss = c.row_loss ? c.row_loss : m.at<float>(l.losses);
 	int* valid = m.at<int>(l.valid);
-	NNB_TRY(split16::find_range(s, c.x, c.P * c.D, xr));
-	NNB_TRY(split16::find_range(s, c.w, c.V * c.D, wr));
-	NNB_TRY(split16::pack(s, c.w, c.V, c.D, (c.V + 2 * kRows - 1) / (2 * kRows) * 2, parts, wr, m.at<void>(l.wpack), nullptr));
+	NNB_CUDA_TRY(cudaMemsetAsync(xr, 0, 2 * sizeof(split16::Range) + (size_t)c.P * sizeof(int), s));
+	NNB_TRY(split16::find_ranges(s, c.x, c.P * c.D, c.w, c.V * c.D, xr));
 	split16::Pack W, X, G;
 	W.buf = m.at<void>(l.wpack); W.rows = c.V; W.cols = c.D;
 	const long long rg = c.P / c.groups;             // parameter gradients are kept per group of rows
@@ -323,9 +330,10 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 			const long long n = std::min(l.piece, (z + 1) * rg - r0), blocks = (n + kRows - 1) / kRows, pad = blocks * kRows;
 			const int first = r0 == z * rg;
 			const float* x = c.x + r0 * c.D;
-			int* x_bad = m.at<int>(l.x_bad);
-			NNB_CUDA_TRY(cudaMemsetAsync(x_bad, 0, (size_t)n * sizeof(int), s));
-			NNB_TRY(split16::pack(s, x, n, c.D, blocks, parts, xr, m.at<void>(l.xpack), x_bad));
+			int* x_bad = m.at<int>(l.x_bad) + r0;
+			const split16::PackJob jobs[2] = {{x, n, c.D, blocks, xr, m.at<void>(l.xpack), x_bad},
+				{c.w, c.V, c.D, (c.V + 2 * kRows - 1) / (2 * kRows) * 2, wr, m.at<void>(l.wpack), nullptr}};
+			NNB_TRY(split16::pack(s, jobs, r0 == 0 ? 2 : 1, parts));           // W with the first piece
 			X.buf = m.at<void>(l.xpack); X.rows = n; X.cols = c.D;
 
 			split16::Product p;
@@ -428,21 +436,32 @@ nnb_status nnb_linear_ce_fwd(void* stream, size_t P, size_t D, size_t V, size_t 
 	return st != NNB_OK ? st : st2;
 }
 
-nnb_status nnb_scaled_accumulate(void* stream, size_t groups, size_t n, const float* src, const float* a, const float* b,
-		float* dst, size_t dst_stride, int first) {
+nnb_status nnb_scaled_accumulate(void* stream, size_t count, const nnb_scaled_grad* grads, const float* a, const float* b) {
 	using namespace nnb;
-	if (n == 0 || groups == 0) return NNB_OK;
-	if (!src || !a || !b || !dst) return fail(NNB_ERR_INVALID, "scaled_accumulate: null pointer");
-	if (groups > 65535) return fail(NNB_ERR_UNSUPPORTED, "scaled_accumulate: more than 65535 groups");
-	const size_t stride = dst_stride ? dst_stride : n;
-	if (groups > 1 && stride < n) return fail(NNB_ERR_INVALID, "scaled_accumulate: the groups overlap");
-	const bool vec = n % 4 == 0 && stride % 4 == 0 &&
-		((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
+	if (count == 0) return NNB_OK;
+	if (count > kScaledMax) return fail(NNB_ERR_UNSUPPORTED, "scaled_accumulate: more than %d tensors", kScaledMax);
+	if (!grads || !a || !b) return fail(NNB_ERR_INVALID, "scaled_accumulate: null pointer");
+	ScaledList l;
+	l.a = a;
+	l.b = b;
+	int used = 0;
+	size_t most = 0;
+	for (size_t i = 0; i < count; ++i) {
+		nnb_scaled_grad e = grads[i];
+		if (e.n == 0 || e.groups == 0) continue;
+		if (!e.src || !e.dst) return fail(NNB_ERR_INVALID, "scaled_accumulate: null pointer in tensor %zu", i);
+		if (e.dst_stride == 0) e.dst_stride = e.n;
+		if (e.groups > 1 && e.dst_stride < e.n) return fail(NNB_ERR_INVALID, "scaled_accumulate: the groups of tensor %zu overlap", i);
+		l.vec[used] = e.n % 4 == 0 && e.dst_stride % 4 == 0 &&
+			((reinterpret_cast<uintptr_t>(e.src) | reinterpret_cast<uintptr_t>(e.dst)) & 15) == 0;
+		l.g[used++] = e;
+		most = std::max(most, e.n);
+	}
+	if (used == 0) return NNB_OK;
 	cudaStream_t s = static_cast<cudaStream_t>(stream);
 	{
 		TraceScope ts(s, kTraceRowwise);
-		scaled_accumulate_kernel<<<dim3(grid_for((long long)(vec ? n / 4 : n), 256), (unsigned)groups), 256, 0, s>>>(
-			(long long)n, src, a, b, dst, (long long)stride, first, vec);
+		scaled_accumulate_kernel<<<dim3(grid_for((long long)(most + 3) / 4, 256), (unsigned)used), 256, 0, s>>>(l);
 	}
 	return cuda_status(cudaGetLastError(), "scaled_accumulate launch");
 }

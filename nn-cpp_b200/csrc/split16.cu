@@ -11,7 +11,7 @@
 // Tensor bound: 3 MMAs per 128 x 256 x 16 step, 1.6 PFLOP/s of fp16 (the measured bf16 burst rate) or 540
 // TFLOP/s of the fp32 product.
 #include <algorithm>
-#include <mutex>
+#include <atomic>
 
 #include "nnb_ops.h"
 #include "nnb_split16.cuh"
@@ -24,7 +24,19 @@ namespace {
 
 // ---- range and pack --------------------------------------------------------------------------
 
-__global__ void __launch_bounds__(256) range_kernel(const float* __restrict__ x, long long n, int vec, Range* out) {
+struct RangeJobs {
+	const float* x[2];
+	long long n[2];
+	int vec[2];
+	Range* out;
+};
+
+// grid.y: the matrix.
+__global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
+	const float* __restrict__ x = jobs.x[blockIdx.y];
+	const long long n = jobs.n[blockIdx.y];
+	const int vec = jobs.vec[blockIdx.y];
+	Range* out = jobs.out + blockIdx.y;
 	unsigned top = 0, bad = 0;
 	auto see = [&](float v) {
 		const unsigned b = __float_as_uint(v) & 0x7fffffffu;
@@ -60,12 +72,29 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 	return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Four columns per thread: a float4 in (or four floats), 8 bytes of hi and of lo out.
-__global__ void __launch_bounds__(256) pack_kernel(const float* __restrict__ x, long long rows, long long cols, long long kw,
-		long long total, int vec, int parts, const Range* __restrict__ range, unsigned char* __restrict__ out,
-		int* __restrict__ row_bad) {
-	const float s = exp2_int(range_shift(range));
-	const long long quads = kw * (kCols / 4);
+struct PackWork {
+	const float* x;
+	long long rows, cols, total;               // total: quads of the padded matrix
+	int vec;
+	const Range* range;
+	unsigned char* out;
+	int* row_bad;
+};
+struct PackJobs {
+	PackWork job[2];
+	int parts;
+};
+
+// Four columns per thread: a float4 in (or four floats), 8 bytes of hi and of lo out. grid.y: the matrix.
+__global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
+	const PackWork& w = jobs.job[blockIdx.y];
+	const float* __restrict__ x = w.x;
+	unsigned char* __restrict__ out = w.out;
+	int* __restrict__ row_bad = w.row_bad;
+	const long long rows = w.rows, cols = w.cols, total = w.total;
+	const int vec = w.vec, parts = jobs.parts;
+	const float s = exp2_int(range_shift(w.range));
+	const long long kw = (cols + kCols - 1) / kCols, quads = kw * (kCols / 4);
 	for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
 		long long r, q;
 		if (total < 0x7fffffffLL) {
@@ -518,7 +547,11 @@ nnb_status map_mn(CUtensorMap* map, const Pack& a, int chunks) {
 template <int kParts, bool kMnA, bool kMnB, int kEpi>
 nnb_status launch(cudaStream_t s, const DeviceState* dev, const Product& p, const CUtensorMap& ta, const CUtensorMap& tb) {
 	auto kernel = split16_kernel<kParts, kMnA, kMnB, kEpi>;
-	NNB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kParts)));
+	static std::atomic<bool> ready[64];                // the attribute holds for the device once set
+	if (!ready[dev->device & 63].load(std::memory_order_relaxed)) {
+		NNB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kParts)));
+		ready[dev->device & 63].store(true, std::memory_order_relaxed);
+	}
 	const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
 	{
 		TraceScope ts(s, kTraceGemm);
@@ -539,24 +572,40 @@ nnb_status dispatch(cudaStream_t s, const DeviceState* dev, int epilogue, bool m
 
 }  // namespace
 
-nnb_status find_range(cudaStream_t s, const float* x, long long n, Range* out) {
-	NNB_CUDA_TRY(cudaMemsetAsync(out, 0, sizeof(Range), s));
-	const bool vec = n % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+nnb_status find_ranges(cudaStream_t s, const float* x0, long long n0, const float* x1, long long n1, Range* out) {
+	RangeJobs jobs;
+	const float* xs[2] = {x0, x1};
+	const long long ns[2] = {n0, n1};
+	for (int i = 0; i < 2; ++i) {
+		jobs.x[i] = xs[i];
+		jobs.n[i] = ns[i];
+		jobs.vec[i] = ns[i] % 4 == 0 && (reinterpret_cast<uintptr_t>(xs[i]) & 15) == 0;
+	}
+	jobs.out = out;
+	const long long n = std::max(n0, n1);
 	{
 		TraceScope ts(s, kTracePack);
-		range_kernel<<<(unsigned)std::min<long long>((n + 4095) / 4096, 148 * 8), 256, 0, s>>>(x, n, vec, out);
+		range_kernel<<<dim3((unsigned)std::min<long long>((n + 4095) / 4096, 148 * 8), 2), 256, 0, s>>>(jobs);
 	}
 	return cuda_status(cudaGetLastError(), "range launch");
 }
 
-nnb_status pack(cudaStream_t s, const float* x, long long rows, long long cols, long long row_blocks, int parts,
-		const Range* range, void* buf, int* row_bad) {
-	const long long kw = (cols + kCols - 1) / kCols, total = row_blocks * kRows * kw * (kCols / 4);
-	const bool vec = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts) {
+	PackJobs k;
+	k.parts = parts;
+	long long most = 0;
+	for (int i = 0; i < count; ++i) {
+		const PackJob& j = jobs[i];
+		PackWork& w = k.job[i];
+		w.x = j.x; w.rows = j.rows; w.cols = j.cols; w.range = j.range;
+		w.out = static_cast<unsigned char*>(j.buf); w.row_bad = j.row_bad;
+		w.total = j.row_blocks * kRows * ((j.cols + kCols - 1) / kCols) * (kCols / 4);
+		w.vec = j.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(j.x) & 15) == 0;
+		most = std::max(most, w.total);
+	}
 	{
 		TraceScope ts(s, kTracePack);
-		pack_kernel<<<(unsigned)std::min<long long>((total + 255) / 256, 148 * 32), 256, 0, s>>>(x, rows, cols, kw, total, vec,
-			parts, range, static_cast<unsigned char*>(buf), row_bad);
+		pack_kernel<<<dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 32), (unsigned)count), 256, 0, s>>>(k);
 	}
 	return cuda_status(cudaGetLastError(), "split pack launch");
 }

@@ -135,7 +135,7 @@ _SIGS = {
     "nnb_residual_norm_bwd": ([_p, _sz, _sz, _sz, _sz, _i, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
                                _p], _i),
     "nnb_linear_ce_fwd": ([_p, _sz, _sz, _sz, _sz, _p, _p, _p, _p, _c.c_int64, _f, _p, _p, _p, _p, _p, _sz, _p, _sz], _i),
-    "nnb_scaled_accumulate": ([_p, _sz, _sz, _p, _p, _p, _p, _sz, _i], _i),
+    "nnb_scaled_accumulate": ([_p, _sz, _p, _p, _p], _i),
     "nnb_manual_seed": ([_c.c_uint64], None),
     "nnb_is_seeded": ([], _i),
     "nnb_seed_epoch": ([], _c.c_uint64),
@@ -159,6 +159,11 @@ _SIGS = {
 class GradOut(_c.Structure):
     """nnb_grad_out: a gradient output of nnb_residual_norm_bwd."""
     _fields_ = [("p", _p), ("stride", _sz), ("first", _i)]
+
+
+class ScaledGrad(_c.Structure):
+    """nnb_scaled_grad: a tensor of nnb_scaled_accumulate."""
+    _fields_ = [("src", _p), ("dst", _p), ("n", _sz), ("groups", _sz), ("dst_stride", _sz), ("first", _i)]
 
 
 NORM_LAYER, NORM_RMS = 0, 1

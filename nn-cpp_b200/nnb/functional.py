@@ -15,12 +15,8 @@ import weakref
 
 import torch
 
-from . import NORM_LAYER, NORM_RMS, GradOut, TensorShapeError, check, lib
-from .autograd import Value, empty
-
-
-def _s():
-    return torch.cuda.current_stream().cuda_stream
+from . import NORM_LAYER, NORM_RMS, GradOut, ScaledGrad, TensorShapeError, check, lib
+from .autograd import Value, current_stream as _s, empty
 
 
 def _p(t):
@@ -393,7 +389,7 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     _check_buffers("residual_norm", (x, branch, gamma, beta, post_gamma, post_beta, gate))
     k = NORM_LAYER if layer else NORM_RMS
     opt = lambda v: None if v is None else v.data.data_ptr()
-    h_data, y_data = empty(x.shape), empty(x.shape)
+    h_data, y_data = torch.empty_like(x.data), torch.empty_like(x.data)
     stream_parents = tuple(v for v in (x, branch, post_gamma, post_beta, gate) if v is not None)
     norm_parents = tuple(v for v in (gamma, beta) if v is not None)
     train = any(_need(v) for v in stream_parents + norm_parents)
@@ -874,12 +870,14 @@ def linear_cross_entropy(x: Value, weight: Value, bias: Value | None, targets: t
                                   _p(db), 0))
 
     def backward(g):
-        k = norm if grad_norm is None else grad_norm
+        grads = []
         for v, d in ((x, dx), (weight, dw), (bias, db)):
             if d is not None:
                 buf, f = v.grad_accum()
                 n = v.data.numel()
-                check(lib().nnb_scaled_accumulate(_s(), d.numel() // n, n, _p(d), _p(g), _p(k), _p(buf), _gstride(buf, v), f))
+                grads.append(ScaledGrad(d.data_ptr(), buf.data_ptr(), n, d.numel() // n, _gstride(buf, v), f))
+        check(lib().nnb_scaled_accumulate(_s(), len(grads), (ScaledGrad * len(grads))(*grads), _p(g),
+                                          _p(norm if grad_norm is None else grad_norm)))
 
     return Value.node(loss, parents, backward)
 

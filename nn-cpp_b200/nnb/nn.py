@@ -414,7 +414,7 @@ class _BatchNorm(Module):
             mu, var = torch.empty(C, device=x.data.device), torch.empty(C, device=x.data.device)
             out = F.batchnorm(x, self.weight, self.bias, self.eps, fuse_relu, mean_out=mu, var_out=var)
             count = x.data.numel() // C
-            check(lib().nnb_batchnorm_running_update(torch.cuda.current_stream().cuda_stream, C, count, mu.data_ptr(),
+            check(lib().nnb_batchnorm_running_update(F._s(), C, count, mu.data_ptr(),
                                                      var.data_ptr(), ctypes.c_float(self.momentum),
                                                      self.running_mean.data_ptr(), self.running_var.data_ptr()))
             return out
@@ -560,7 +560,7 @@ class AdamW:
             self.offsets.append(self.offsets[-1] + -(-n // self.BLOCK) * self.BLOCK)
         total = self.offsets[-1]
         dev = self.params[0].data.device if self.params else None
-        s = torch.cuda.current_stream().cuda_stream
+        s = F._s()
 
         def zeros(count, dtype):
             t = torch.empty(count, dtype=dtype, device=dev)
@@ -590,7 +590,7 @@ class AdamW:
         if self.state_bits == 32:
             return self.flat_m, self.flat_v
         m, v = (torch.empty(self.offsets[-1], dtype=torch.float32, device=self.flat_m.device) for _ in range(2))
-        check(lib().nnb_adamw8_moments(torch.cuda.current_stream().cuda_stream, m.numel(), self.flat_m.data_ptr(),
+        check(lib().nnb_adamw8_moments(F._s(), m.numel(), self.flat_m.data_ptr(),
                                        self.flat_v.data_ptr(), self.unit_m.data_ptr(), self.unit_v.data_ptr(),
                                        m.data_ptr(), v.data_ptr()))
         return m, v
@@ -656,7 +656,7 @@ class AdamW:
         if not self.params:
             self.t += 1
             return
-        s = torch.cuda.current_stream().cuda_stream
+        s = F._s()
         for p in self.params:
             if p.grad_fresh:     # nothing reached this parameter: its gradient is all zeros
                 check(lib().nnb_fill(s, p.grad.numel(), 0.0, p.grad.data_ptr()))

@@ -30,13 +30,15 @@ def test_refusals():
 
 
 def test_scaled_accumulate_refusals():
-    f = nnb.lib().nnb_scaled_accumulate
-    assert f(None, 0, 4, None, None, None, None, 0, 1) == nnb.NNB_OK
-    assert f(None, 2, 0, None, None, None, None, 0, 1) == nnb.NNB_OK
-    for i in range(4):
-        assert f(None, 1, 4, *[None if j == i else P for j in range(4)], 0, 1) == nnb.NNB_ERR_INVALID
-    assert f(None, 2, 4, P, P, P, P, 3, 1) == nnb.NNB_ERR_INVALID
-    assert f(None, 70000, 4, P, P, P, P, 0, 1) == nnb.NNB_ERR_UNSUPPORTED
+    def call(*entries, a=P, b=P):
+        return nnb.lib().nnb_scaled_accumulate(None, len(entries), (nnb.ScaledGrad * max(1, len(entries)))(*entries), a, b)
+    good = nnb.ScaledGrad(P, P, 4, 1, 0, 1)
+    assert call() == nnb.NNB_OK
+    assert call(nnb.ScaledGrad(None, None, 0, 1, 0, 1), nnb.ScaledGrad(None, None, 4, 0, 0, 1)) == nnb.NNB_OK
+    for bad in (nnb.ScaledGrad(None, P, 4, 1, 0, 1), nnb.ScaledGrad(P, None, 4, 1, 0, 1), nnb.ScaledGrad(P, P, 4, 2, 3, 1)):
+        assert call(good, bad) == nnb.NNB_ERR_INVALID and "tensor 1" in nnb.last_error()
+    assert call(good, a=None) == nnb.NNB_ERR_INVALID and call(good, b=None) == nnb.NNB_ERR_INVALID
+    assert call(*[good] * 9) == nnb.NNB_ERR_UNSUPPORTED
 
 
 @pytest.mark.parametrize("op", [F.linear_cross_entropy, F.linear_token_losses])
