@@ -405,7 +405,7 @@ nnb_status check_list(const char* who, size_t count, const size_t* n, float* con
 		if (n[i] == 0) continue;
 		if (!w[i] || !a.m[i] || !a.v[i] || (units && (!a.mu[i] || !a.vu[i])))
 			return fail(NNB_ERR_INVALID, "%s: null pointer in tensor %zu", who, i);
-		if (n[i] > (size_t(1) << 42)) return fail(NNB_ERR_UNSUPPORTED, "%s: tensor %zu is too large", who, i);
+		if (n[i] > (size_t(1) << 40)) return fail(NNB_ERR_UNSUPPORTED, "%s: tensor %zu is too large", who, i);
 	}
 	return NNB_OK;
 }

@@ -417,6 +417,9 @@ nnb_status nnb_linear_ce_fwd(void* stream, size_t P, size_t D, size_t V, size_t 
 		return fail(NNB_ERR_INVALID, "%s: the groups' gradients overlap", who);
 	if (P > (size_t(1) << 31) - 1 || V > (size_t(1) << 30) || D > (size_t(1) << 30))
 		return fail(NNB_ERR_UNSUPPORTED, "%s: dimension too large", who);
+	// packed rows of w and x that a tensor map can count
+	if ((V + 255) / 256 * 256 * ((D + 63) / 64) * 2 > INT32_MAX || (P + 127) / 128 * 128 * ((D + 63) / 64) * 2 > INT32_MAX)
+		return fail(NNB_ERR_UNSUPPORTED, "%s: more packed rows than a tensor map holds", who);
 	DeviceState* dev = nullptr;
 	NNB_TRY(device_state(&dev));
 	cudaStream_t s = static_cast<cudaStream_t>(stream);

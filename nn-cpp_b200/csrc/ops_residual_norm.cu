@@ -216,7 +216,7 @@ nnb_status check_common(const char* who, size_t R, size_t D, size_t gate_rows, i
 	if (kind != NNB_NORM_LAYER && kind != NNB_NORM_RMS) return fail(NNB_ERR_INVALID, "%s: unknown norm %d", who, kind);
 	if (D == 0) return fail(NNB_ERR_SHAPE, "%s: empty rows", who);
 	if (D > kMaxD) return fail(NNB_ERR_UNSUPPORTED, "%s: rows of %zu values, at most %d", who, D, kMaxD);
-	if (R >= (size_t(1) << 40)) return fail(NNB_ERR_UNSUPPORTED, "%s: too many rows", who);
+	if (R > (size_t(1) << 31) - 1) return fail(NNB_ERR_UNSUPPORTED, "%s: too many rows", who);
 	if (!gamma) return fail(NNB_ERR_INVALID, "%s: gamma is null", who);
 	if (beta_given && (kind == NNB_NORM_LAYER) != (beta != nullptr))
 		return fail(NNB_ERR_INVALID, "%s: a layer norm needs a beta, an rms norm has none", who);

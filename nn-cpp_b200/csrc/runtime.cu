@@ -139,7 +139,11 @@ nnb_status encode_tiled_2d(CUtensorMap* map, const void* base, uint64_t inner, u
 nnb_status scratch_alloc(void** p, size_t bytes, cudaStream_t s) {
 	*p = nullptr;
 	if (bytes == 0) return NNB_OK;
-	NNB_CUDA_TRY(cudaMallocAsync(p, bytes, s));
+	const cudaError_t e = cudaMallocAsync(p, bytes, s);
+	if (e != cudaSuccess) {
+		(void)cudaGetLastError();              // out of memory is not the next launch's error
+		return fail(NNB_ERR_CUDA, "%zu bytes of scratch memory: %s", bytes, cudaGetErrorString(e));
+	}
 	return NNB_OK;
 }
 

@@ -26,6 +26,7 @@ def test_refusals():
         assert _fwd(**{k: None}) == INV, k
     assert _fwd(bias=None) == INV and "bias" in nnb.last_error()
     assert _fwd(groups=2, dws=63) == INV and _fwd(groups=2, dbs=7) == INV and "overlap" in nnb.last_error()
+    assert _fwd(V=2 ** 28, D=2 ** 10) == UNSUP and "tensor map" in nnb.last_error()
     assert _fwd(rows=2 ** 31) == UNSUP and _fwd(V=2 ** 31) == UNSUP and _fwd(D=2 ** 31) == UNSUP
 
 

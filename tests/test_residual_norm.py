@@ -31,7 +31,7 @@ def test_forward_refusals():
     assert _fwd(kind=2) == INV and "unknown norm" in nnb.last_error()
     assert _fwd(D=0) == SHAPE
     assert _fwd(D=16385) == UNSUP and "16384" in nnb.last_error()
-    assert _fwd(R=2 ** 41) == UNSUP
+    assert _fwd(R=2 ** 31) == UNSUP
     for name in ("x", "branch", "gamma", "beta", "h", "y"):        # (branch and h go together)
         assert _fwd(**{name: None}) == INV, name
     assert _fwd(branch=None, h=None, gate=P, gate_rows=1) == INV and _fwd(branch=None, h=None, pg=P, pb=P) == INV
