@@ -13,6 +13,7 @@ torch provides allocation and streams only; every number is produced by a kernel
 """
 from __future__ import annotations
 
+import functools
 from typing import Callable, Sequence
 
 import torch
@@ -25,9 +26,14 @@ def current_stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+@functools.cache
+def _device(index: int) -> torch.device:
+    return torch.device("cuda", index)
+
+
 def empty(shape, dtype=torch.float32, device=None):
     """An uninitialised device buffer (plumbing: no kernel runs)."""
-    return torch.empty(shape, dtype=dtype, device=torch.cuda.current_device() if device is None else device)
+    return torch.empty(shape, dtype=dtype, device=_device(torch.cuda.current_device()) if device is None else device)
 
 
 _ONES: dict = {}
@@ -122,23 +128,25 @@ def backward(roots: Sequence[Value], seeds: Sequence[torch.Tensor | None]) -> No
             raise ValueError("backward() needs a single-element value (AutogradShapeError)")
         if seed is not None and seed.numel() != root.data.numel():
             raise ValueError("backward(): the seed must have the root's element count")
+        if seed is not None and (seed.dtype is not root.data.dtype or seed.device != root.data.device):
+            raise ValueError("backward(): the seed must have the root's type and device")
+    # iterative post-order walk over the values that have a rule (a value without one has no parents)
     topo: list[Value] = []
-    expanded, done = set(), set()
+    done: dict[int, bool] = {}               # False: its parents are on the stack; True: in topo
     stack = list(roots)
     while stack:
         v = stack[-1]
-        if id(v) in done:
-            stack.pop()
+        seen = done.get(id(v))
+        if seen is None:
+            done[id(v)] = False
+            for p in v.parents:
+                if p.backward_fn is not None and id(p) not in done:
+                    stack.append(p)
             continue
-        if id(v) in expanded:
-            stack.pop()
-            done.add(id(v))
+        stack.pop()
+        if not seen:
+            done[id(v)] = True
             topo.append(v)
-            continue
-        expanded.add(id(v))
-        for p in v.parents:
-            if id(p) not in expanded:
-                stack.append(p)
     seeded = {id(r) for r in roots}
     for v in topo:
         if v.backward_fn is not None and id(v) not in seeded:
@@ -147,8 +155,7 @@ def backward(roots: Sequence[Value], seeds: Sequence[torch.Tensor | None]) -> No
                 v.grad_borrowed = False
             v.grad_fresh = True
     for root, seed in zip(roots, seeds):
-        if seed is None:
-            seed = _one(root.data.device)
+        seed = _one(root.data.device) if seed is None else seed.contiguous()
         root.grad = seed if seed.shape == root.data.shape else seed.view(root.data.shape)
         root.grad_fresh, root.grad_borrowed = False, True
     for v in reversed(topo):

@@ -342,10 +342,15 @@ def layernorm(x: Value, gamma: Value, beta: Value, eps: float) -> Value:
 
 def _check_buffers(who: str, values, dtype=torch.float32) -> None:
     """Refuses values that are not contiguous buffers of `dtype` on the current CUDA device (None: skipped)."""
-    tensors = [v.data if isinstance(v, Value) else v for v in values if v is not None]
-    dev = torch.cuda.current_device() if all(t.is_cuda for t in tensors) else None
-    for t in tensors:
-        if t.get_device() != dev:
+    dev = None
+    for v in values:
+        if v is None:
+            continue
+        t = v.data if isinstance(v, Value) else v
+        at = t.get_device()
+        if dev is None and at >= 0:
+            dev = torch.cuda.current_device()
+        if at != dev:
             raise ValueError(f"{who}: tensors must be on the current CUDA device, one is on {t.device}")
         if t.dtype is not dtype or not t.is_contiguous():
             raise ValueError(f"{who}: tensors must be contiguous {dtype}, one is {t.dtype}")
@@ -369,14 +374,16 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     if kind not in ("layer", "rms"):
         raise ValueError('residual_norm: kind must be "layer" or "rms"')
     layer = kind == "layer"
-    if not x.shape or 0 in x.shape or branch.shape != x.shape:
+    shape = x.data.shape
+    if not shape or 0 in shape or branch.data.shape != shape:
         raise TensorShapeError("residual_norm: x and branch need one non-empty shape")
-    D = x.shape[-1]
+    D = shape[-1]
     R = x.data.numel() // D
     if layer != (beta is not None) or (post_beta is not None) != (layer and post_gamma is not None):
         raise ValueError("residual_norm: a layer norm needs a beta, an rms norm has none")
-    if any(p is not None and p.shape != (D,) for p in (gamma, beta, post_gamma, post_beta)):
-        raise TensorShapeError("residual_norm: norm parameters must be [D]")
+    for p in (gamma, beta, post_gamma, post_beta):
+        if p is not None and p.data.shape != (D,):
+            raise TensorShapeError("residual_norm: norm parameters must be [D]")
     gate_rows = 0
     if gate is not None:
         if not gate.shape or gate.shape[-1] != D or gate.data.numel() == 0 or R % (gate.data.numel() // D):
@@ -393,7 +400,7 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     stream_parents = tuple(v for v in (x, branch, post_gamma, post_beta, gate) if v is not None)
     norm_parents = tuple(v for v in (gamma, beta) if v is not None)
     train = any(_need(v) for v in stream_parents + norm_parents)
-    stats = empty((R, 4)) if train else None
+    stats = x.data.new_empty((R, 4)) if train else None
     check(lib().nnb_residual_norm_fwd(_s(), R, D, gate_rows, k, eps, scale, _p(x.data), _p(branch.data), opt(post_gamma),
                                       opt(post_beta), opt(gate), _p(gamma.data), opt(beta), _p(h_data), _p(y_data),
                                       _p(stats)))

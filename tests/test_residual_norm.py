@@ -104,3 +104,5 @@ def test_backward_from_several_roots_refusals():
         backward((b, a), (None, None))
     with pytest.raises(ValueError, match="element count"):
         backward((a,), (torch.zeros(3),))
+    with pytest.raises(ValueError, match="type and device"):
+        backward((a,), (torch.zeros(2, dtype=torch.float64),))

@@ -302,6 +302,14 @@ def test_seeds_are_not_written(cuda):
     assert all(torch.equal(vals[k].grad, want[k]) for k in want)
 
 
+def test_seeds_of_any_strides(cuda):
+    ops, _, _ = _make(10, 32, 10, "layer", False, "none", seed=16)
+    dh, dy = torch.ones(1, device="cuda").expand(10, 32), torch.randn(32, 10, device="cuda").t()
+    want = _run(ops, dh.clone(memory_format=torch.contiguous_format), dy.contiguous(), "layer", 1.0)[2]
+    got = _run(ops, dh, dy, "layer", 1.0)[2]
+    assert all(torch.equal(got[k], want[k]) for k in want)
+
+
 def test_captured_and_on_another_stream(cuda):
     ops, dh, dy = _make(400, 512, 100, "rms", True, "sequence", seed=14)
     want = _run(ops, dh, dy, "rms", 1.0)
