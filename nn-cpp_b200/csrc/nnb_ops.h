@@ -30,4 +30,24 @@ inline unsigned grid_for(long long n, int threads) {
 	return (unsigned)b;
 }
 
+// Launches a kernel of a chain: it may start while the stream's previous kernel still runs, as far as its
+// chain_wait (nnb_ptx.cuh), which it calls before it touches memory. Its launch and prologue then hide behind
+// the previous kernel, about 2 us of each step of a chain of short kernels.
+template <typename... P, typename... A>
+cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, A&&... args) {
+	cudaLaunchConfig_t c = {};
+	c.gridDim = grid;
+	c.blockDim = dim3(threads);
+	c.dynamicSmemBytes = smem;
+	c.stream = s;
+	cudaLaunchAttribute a[1];
+	a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	a[0].val.programmaticStreamSerializationAllowed = 1;
+	c.attrs = a;
+	c.numAttrs = 1;
+	const cudaError_t e = cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+	if (e != cudaSuccess) (void)cudaGetLastError();      // returned here, not left for the next check
+	return e;
+}
+
 }  // namespace nnb

@@ -335,6 +335,14 @@ __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t
 		: "memory");
 }
 
+// A chained kernel's first step (launch_chained): lets the next kernel of the chain be launched as soon as
+// every CTA of this one has got here, then waits until the previous kernel has finished and its writes are
+// visible. Nothing before it may touch memory that an earlier kernel writes or reads.
+__device__ __forceinline__ void chain_wait() {
+	asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+	asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Barrier over `count` threads (a multiple of 32) with id 1..15; id 0 is __syncthreads.
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t count) {
 	asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");

@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const float2* __restrict__
 	__shared__ float2 ms[32][9];
 	__shared__ float tot[32][9];
 	const int x = threadIdx.x & 7, y = threadIdx.x >> 3, r = blockIdx.x * 8 + x;
+	chain_wait();
 	float top = -INFINITY, sum = 0.0f, total = 0.0f;
 	// (an empty part is (-inf, 0); a NaN or infinite logit leaves a NaN sum, and so does +inf as a maximum)
 	auto join = [&](float2 b) {
@@ -113,6 +114,7 @@ __global__ void __launch_bounds__(256) ce_grad_kernel(float* __restrict__ blocks
 	float* block = blocks + ((long long)rb * kw + c64) * (kRows * kCols);
 	const int col = c64 * kCols + q * 4;
 	const float spread = ls / (float)V, scale = exp2f((float)kGShift);
+	chain_wait();
 	float4 l[8];
 	RowInfo in[8];
 #pragma unroll
@@ -173,6 +175,7 @@ __global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ 
 		float* __restrict__ db, int first) {
 	__shared__ float tile[8][32];
 	const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+	chain_wait();
 	float s = 0.0f;
 	if (c < V)
 #pragma unroll 8
@@ -191,6 +194,7 @@ __global__ void __launch_bounds__(1024) ce_mean_kernel(long long rows, const flo
 	__shared__ double sums[32];
 	__shared__ long long counts[32];
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	chain_wait();
 	double s = 0.0;
 	long long n = 0;
 	for (long long r = threadIdx.x; r < rows; r += 1024) {
@@ -351,24 +355,22 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 			RowInfo* info = c.grad() ? m.at<RowInfo>(l.info) : nullptr;
 			{
 				TraceScope ts(s, kTraceRowwise);
-				ce_rows_kernel<<<(unsigned)(pad / 8), 256, 0, s>>>(p.part, p.part_sum, p.target_logit, (int)c.parts(), (int)n,
-					(int)pad, (int)c.V, p.targets, c.ignore_index, c.ls, x_bad, wr, row_loss + r0, valid + r0, info,
-					dev->error_word);
+				NNB_CUDA_TRY(launch_chained(ce_rows_kernel, (unsigned)(pad / 8), 256, 0, s, p.part, p.part_sum, p.target_logit,
+					(int)c.parts(), (int)n, (int)pad, (int)c.V, p.targets, c.ignore_index, c.ls, x_bad, wr, row_loss + r0,
+					valid + r0, info, dev->error_word));
 			}
-			NNB_TRY(cuda_status(cudaGetLastError(), "linear_ce rows launch"));
 			if (c.grad()) {
 				float* cols = c.db ? m.at<float>(l.cols) : nullptr;
 				{
 					TraceScope ts(s, kTraceRowwise);
-					ce_grad_kernel<<<dim3((unsigned)c.kw(), (unsigned)blocks), 256, 0, s>>>(p.blocks, (int)c.kw(), (int)c.V, (int)pad,
-						info, c.ls, parts == 2, cols);
+					NNB_CUDA_TRY(launch_chained(ce_grad_kernel, dim3((unsigned)c.kw(), (unsigned)blocks), 256, 0, s, p.blocks,
+						(int)c.kw(), (int)c.V, (int)pad, info, c.ls, (int)(parts == 2), cols));
 				}
 				if (c.db) {
 					TraceScope ts(s, kTraceRowwise);
-					ce_bias_kernel<<<(unsigned)((c.V + 31) / 32), 256, 0, s>>>(cols, (int)blocks, (int)(c.kw() * kCols), (int)c.V,
-						c.db + z * c.db_stride, first);
+					NNB_CUDA_TRY(launch_chained(ce_bias_kernel, (unsigned)((c.V + 31) / 32), 256, 0, s, cols, (int)blocks,
+						(int)(c.kw() * kCols), (int)c.V, c.db + z * c.db_stride, first));
 				}
-				NNB_TRY(cuda_status(cudaGetLastError(), "linear_ce gradient launch"));
 				G.buf = m.at<void>(l.g); G.rows = n; G.cols = c.V;
 			}
 			// a product cut along its depth leaves its pieces in slabs, summed in order
@@ -391,9 +393,9 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 	}
 	{
 		TraceScope ts(s, kTraceRowwise);
-		ce_mean_kernel<<<1, 1024, 0, s>>>(c.P, row_loss, valid, c.loss, c.norm);
+		NNB_CUDA_TRY(launch_chained(ce_mean_kernel, 1, 1024, 0, s, c.P, row_loss, valid, c.loss, c.norm));
 	}
-	return cuda_status(cudaGetLastError(), "linear_ce mean launch");
+	return NNB_OK;
 }
 
 }  // namespace

@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 	const long long n = jobs.n[blockIdx.y];
 	const int vec = jobs.vec[blockIdx.y];
 	Range* out = jobs.out + blockIdx.y;
+	chain_wait();
 	unsigned top = 0, bad = 0;
 	auto see = [&](float v) {
 		const unsigned b = __float_as_uint(v) & 0x7fffffffu;
@@ -93,6 +94,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
 	int* __restrict__ row_bad = w.row_bad;
 	const long long rows = w.rows, cols = w.cols, total = w.total;
 	const int vec = w.vec, parts = jobs.parts;
+	chain_wait();
 	const float s = exp2_int(range_shift(w.range));
 	const long long kw = (cols + kCols - 1) / kCols, quads = kw * (kCols / 4);
 	for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
@@ -225,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
+	chain_wait();
 	const uint32_t tmem_base = tmem_base_sh;
 	volatile int* abort_flag = &abort_sh;
 	const int items = p.tiles_m * p.tiles_n * p.splits;
@@ -502,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 // c (+)= sum over slabs, in order; four floats per thread where aligned.
 __global__ void __launch_bounds__(256) sum_slabs_kernel(const float* __restrict__ slabs, int splits, long long n,
 		float* __restrict__ c, int accumulate, int vec) {
+	chain_wait();
 	const long long step = gridDim.x * 256LL;
 	long long i = blockIdx.x * 256LL + threadIdx.x;
 	if (vec) {
@@ -555,9 +559,10 @@ nnb_status launch(cudaStream_t s, const DeviceState* dev, const Product& p, cons
 	const long long items = (long long)p.tiles_m * p.tiles_n * p.splits;
 	{
 		TraceScope ts(s, kTraceGemm);
-		kernel<<<(unsigned)std::min<long long>(items, dev->sm_count), kThreads, smem_bytes(kParts), s>>>(ta, tb, p);
+		NNB_CUDA_TRY(launch_chained(kernel, (unsigned)std::min<long long>(items, dev->sm_count), kThreads, smem_bytes(kParts), s,
+			ta, tb, p));
 	}
-	return cuda_status(cudaGetLastError(), "split product launch");
+	return NNB_OK;
 }
 
 template <int kParts>
@@ -585,9 +590,10 @@ nnb_status find_ranges(cudaStream_t s, const float* x0, long long n0, const floa
 	const long long n = std::max(n0, n1);
 	{
 		TraceScope ts(s, kTracePack);
-		range_kernel<<<dim3((unsigned)std::min<long long>((n + 4095) / 4096, 148 * 8), 2), 256, 0, s>>>(jobs);
+		NNB_CUDA_TRY(launch_chained(range_kernel, dim3((unsigned)std::min<long long>((n + 4095) / 4096, 148 * 8), 2), 256, 0, s,
+			jobs));
 	}
-	return cuda_status(cudaGetLastError(), "range launch");
+	return NNB_OK;
 }
 
 nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts) {
@@ -605,9 +611,10 @@ nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts) {
 	}
 	{
 		TraceScope ts(s, kTracePack);
-		pack_kernel<<<dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 32), (unsigned)count), 256, 0, s>>>(k);
+		NNB_CUDA_TRY(launch_chained(pack_kernel, dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 32), (unsigned)count),
+			256, 0, s, k));
 	}
-	return cuda_status(cudaGetLastError(), "split pack launch");
+	return NNB_OK;
 }
 
 // Chunks of 128 terms in a depth of K.
@@ -666,9 +673,10 @@ nnb_status sum_slabs(cudaStream_t s, const float* slabs, int splits, long long n
 	const bool vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(slabs) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
 	{
 		TraceScope ts(s, kTraceAux);
-		sum_slabs_kernel<<<grid_for(vec ? n / 4 : n, 256), 256, 0, s>>>(slabs, splits, n, c, accumulate, vec);
+		NNB_CUDA_TRY(launch_chained(sum_slabs_kernel, grid_for(vec ? n / 4 : n, 256), 256, 0, s, slabs, splits, n, c, accumulate,
+			(int)vec));
 	}
-	return cuda_status(cudaGetLastError(), "slab sum launch");
+	return NNB_OK;
 }
 
 }  // namespace split16
