@@ -868,23 +868,30 @@ def linear_cross_entropy(x: Value, weight: Value, bias: Value | None, targets: t
     groups = _GROUPS if params else 1
     if P % groups:
         raise TensorShapeError("linear_cross_entropy: the rows do not divide into the parameter groups")
-    loss, norm = empty((1,)), empty((1,))
-    dx = empty((P, D)) if _need(x) else None
-    dw = empty((groups, V, D)) if _need(weight) else None
-    db = empty((groups, V)) if bias is not None and _need(bias) else None
+    # the gradients wanted and the loss' norm in one buffer, each on a 256-byte boundary
+    sizes = [n if v is not None and _need(v) else 0 for v, n in ((x, P * D), (weight, groups * V * D), (bias, groups * V))]
+    starts, total = [], 64
+    for n in sizes:
+        starts.append(total)
+        total += -(-n // 64) * 64
+    loss, kept = x.data.new_empty(1), x.data.new_empty(total)
+    norm_at = kept.data_ptr()
+    at = [norm_at + 4 * lo if n else None for lo, n in zip(starts, sizes)]
     check(lib().nnb_linear_ce_fwd(_s(), P, D, V, groups, _p(x.data), _p(weight.data), None if bias is None else _p(bias.data),
-                                  _p(targets), ignore_index, label_smoothing, None, _p(loss), _p(norm), _p(dx), _p(dw), 0,
-                                  _p(db), 0))
+                                  _p(targets), ignore_index, label_smoothing, None, _p(loss), norm_at, at[0], at[1],
+                                  0, at[2], 0))
 
     def backward(g):
         grads = []
-        for v, d in ((x, dx), (weight, dw), (bias, db)):
-            if d is not None:
+        for v, n, lo in zip((x, weight, bias), sizes, starts):
+            if n:
                 buf, f = v.grad_accum()
-                n = v.data.numel()
-                grads.append(ScaledGrad(d.data_ptr(), buf.data_ptr(), n, d.numel() // n, _gstride(buf, v), f))
-        check(lib().nnb_scaled_accumulate(_s(), len(grads), (ScaledGrad * len(grads))(*grads), _p(g),
-                                          _p(norm if grad_norm is None else grad_norm)))
+                own = v.data.numel()
+                grads.append(ScaledGrad(kept.data_ptr() + 4 * lo, buf.data_ptr(), own, n // own, _gstride(buf, v), f))
+        k = norm_at if grad_norm is None else grad_norm.data_ptr()
+        # (one launch, unless x is the weight itself: then its two gradients are added one after the other)
+        for part in ([grads] if x is not weight else [[e] for e in grads]):
+            check(lib().nnb_scaled_accumulate(_s(), len(part), (ScaledGrad * len(part))(*part), _p(g), k))
 
     return Value.node(loss, parents, backward)
 

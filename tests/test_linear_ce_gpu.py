@@ -182,6 +182,16 @@ def test_any_subset_needs_gradients(cuda):
         assert torch.equal(part.data, loss) and torch.equal(vals[only].grad, full[only]), only
 
 
+def test_weight_as_input(cuda):
+    """x and the weight are one Value: it receives the sum of both gradients."""
+    _, w, b, _ = _make(1, 40, 64, seed=14)
+    t = torch.arange(64, device="cuda") % 60
+    want = _run(w.clone(), w, b, t)[1]
+    both = Value.leaf(w, True)
+    F.linear_cross_entropy(both, both, Value.leaf(b, False), t).backward()
+    assert torch.equal(both.grad, want["x"] + want["w"])
+
+
 def test_all_ignored_and_bad_targets(cuda):
     x, w, b, t = _make(20, 16, 30, seed=7)
     loss, grads = _run(x, w, b, torch.full_like(t, IGNORE))
