@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "nnb_internal.h"
+#include "nnb_ops.h"
 #include "nnb_ptx.cuh"
 
 namespace nnb {
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 		if constexpr (kStaged == 4) copy(3, p.branch);
 		cp_async_commit();
 	};
+	chain_wait();
 	const long long q = blockIdx.x * (long long)kSlots + slot;
 	long long lo = 0, hi = 0;
 	if (q < p.runs) run_rows(p, q, lo, hi);
@@ -389,8 +391,8 @@ nnb_status launch_bwd(cudaStream_t s, const Grad& p, long long groups) {
 	auto kernel = residual_norm_bwd_kernel<VEC, KV, T, kLayer, kPost, kGate>;
 	if (smem > 40 * 1024)                          // with the static part: above the default 48 KB
 		NNB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-	kernel<<<dim3((unsigned)p.chunks, (unsigned)groups), kThreads, smem, s>>>(p);
-	return cuda_status(cudaGetLastError(), "residual_norm_bwd launch");
+	return cuda_status(launch_chained(kernel, dim3((unsigned)p.chunks, (unsigned)groups), kThreads, smem, s, p),
+		"residual_norm_bwd launch");
 }
 
 // By the threads of a row that the host chose (p.T): eight columns per thread, 16 above 8192.

@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta) residual_norm_fwd_kernel(
 	__shared__ float2 buf[2 * 32];
 	const int slot = threadIdx.x / T, t = threadIdx.x % T;
 	const long long r = blockIdx.x * (long long)kSlots + slot;
+	chain_wait();
 	if (r >= p.rows) return;                       // whole slots leave: the barriers are per slot
 	SlotSum sum(buf, T);
 	const int j0 = t * VEC;
@@ -162,6 +163,7 @@ __global__ void __launch_bounds__(256) residual_norm_params_kernel(const float* 
 	float* out = o.out[array];
 	if (!out) return;
 	const int j = blockIdx.x * 32 + lane;
+	chain_wait();
 	const float* src = part + (array * (long long)gridDim.y + blockIdx.y) * chunks * D + j;
 	float s = 0.0f;
 	if (j < D) {
@@ -189,6 +191,7 @@ __global__ void __launch_bounds__(256) residual_norm_params_kernel(const float* 
 __global__ void residual_norm_gate_kernel(const float* __restrict__ part, long long spans, int pieces, int D,
 		float* __restrict__ dgate, int first) {
 	const long long total = spans * D;
+	chain_wait();
 	for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
 		const long long s = i / D;
 		const float* src = part + s * pieces * D + (i - s * D);
@@ -231,8 +234,8 @@ nnb_status check_common(const char* who, size_t R, size_t D, size_t gate_rows, i
 template <int VEC, int KV, int T>
 nnb_status launch_fwd(cudaStream_t s, const Row& p) {
 	constexpr int kThreads = T > kCta ? T : kCta, kSlots = kThreads / T;
-	residual_norm_fwd_kernel<VEC, KV, T><<<(unsigned)((p.rows + kSlots - 1) / kSlots), kThreads, 0, s>>>(p);
-	return cuda_status(cudaGetLastError(), "residual_norm_fwd launch");
+	NNB_CUDA_TRY(launch_chained(residual_norm_fwd_kernel<VEC, KV, T>, (unsigned)((p.rows + kSlots - 1) / kSlots), kThreads, 0, s, p));
+	return NNB_OK;
 }
 
 // The fewest threads that leave each at most VEC * KV columns; rows that one warp holds with fewer take
@@ -377,15 +380,14 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 	}
 	if (st == NNB_OK && any) {
 		TraceScope ts(s, kTraceRowwise);
-		residual_norm_params_kernel<<<dim3((unsigned)((D + 31) / 32), (unsigned)groups, (unsigned)arrays), 256, 0, s>>>(p.part,
-			p.chunks, p.D, o);
-		st = cuda_status(cudaGetLastError(), "residual_norm_params launch");
+		st = cuda_status(launch_chained(residual_norm_params_kernel,
+			dim3((unsigned)((D + 31) / 32), (unsigned)groups, (unsigned)arrays), 256, 0, s, p.part, p.chunks, p.D, o),
+			"residual_norm_params launch");
 	}
 	if (st == NNB_OK && gate_pieces && p.dgate) {
 		TraceScope ts(s, kTraceRowwise);
-		residual_norm_gate_kernel<<<grid_for((long long)gate_rows * p.D, 256), 256, 0, s>>>(p.gate_part, (long long)gate_rows,
-			(int)p.pieces, p.D, p.dgate, p.dgate_first);
-		st = cuda_status(cudaGetLastError(), "residual_norm_gate launch");
+		st = cuda_status(launch_chained(residual_norm_gate_kernel, grid_for((long long)gate_rows * p.D, 256), 256, 0, s,
+			p.gate_part, (long long)gate_rows, (int)p.pieces, p.D, p.dgate, p.dgate_first), "residual_norm_gate launch");
 	}
 	const nnb_status st2 = scratch_free(ws, s);
 	return st != NNB_OK ? st : st2;
