@@ -75,8 +75,6 @@ struct Product {
 	int a_kw = 0, b_kw = 0;           // packed columns of the operands
 	const Range *ra = nullptr, *rb = nullptr;   // ranges that scale acc back (null: none); see `shift`
 	int shift = 0;                    // acc is also multiplied by 2^-shift
-	const float *row_scale = nullptr, *col_scale = nullptr;   // kStats: or by these, per row and column of C
-	                                  // (both or neither, for the rows and columns of whole tiles)
 	// kStore
 	float* C = nullptr;
 	long long ldc = 0, slab = 0;
@@ -106,18 +104,6 @@ struct PackJob {
 };
 // One or two of them in one launch.
 nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts);
-// The same with every row scaled by its own largest magnitude, found on the way: 1 / its scale goes to
-// scale[row] (row_blocks * 128 of them); `bad` (nullable) is set when any value is not finite. For operands
-// whose rows are never a depth (one read of the matrix instead of two).
-struct RowPackJob {
-	const float* x;
-	long long rows, cols, row_blocks;
-	void* buf;
-	float* scale;
-	int* row_bad;
-	unsigned* bad;
-};
-nnb_status pack_rows(cudaStream_t s, const RowPackJob* jobs, int count, int parts);
 
 // C = A B^T with A = a (K-major: rows of a) or a^T (mn_a: columns of a), B likewise; p's sizes, operands'
 // widths and tile counts are filled in here. parts: 2 or 1.

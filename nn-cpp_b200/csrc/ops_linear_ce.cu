@@ -13,7 +13,7 @@
 // backward pass would cost 8. The backward pass only scales the gradients by the upstream gradient over
 // the number of rows that count, which is known at the end.
 //
-// Ranges (split16): X and W are scaled by their largest magnitude (for the loss alone, each row by its own), G by 2^15 (|G| <= 1): an entry of G below
+// Ranges (split16): X and W are scaled by their largest magnitude, G by 2^15 (|G| <= 1): an entry of G below
 // 2^-17 loses relative precision, down to an absolute 2^-40, next to the -1 of its row's target.
 #include <algorithm>
 #include <cmath>
@@ -291,7 +291,7 @@ struct Scratch {
 struct Layout {
 	long long piece, blocks;                  // rows of a piece, and their 128-row blocks
 	int dx_splits, dw_splits;                 // depth splits of the gradients' products
-	size_t ranges, wpack, xpack, x_bad, w_scale, x_scale, g, part, part_sum, target_logit, info, losses, valid, cols, slabs;
+	size_t ranges, wpack, xpack, x_bad, g, part, part_sum, target_logit, info, losses, valid, cols, slabs;
 };
 
 Layout plan(const Call& c, Scratch& s) {
@@ -305,8 +305,6 @@ Layout plan(const Call& c, Scratch& s) {
 	l.x_bad = l.ranges + 2 * sizeof(split16::Range);
 	l.wpack = s.take(split16::pack_bytes(c.V, c.D));
 	l.xpack = s.take(split16::pack_bytes(l.piece, c.D));
-	l.w_scale = s.take(c.grad() ? 0 : (size_t)(c.V + 255) / 256 * 256 * sizeof(float));
-	l.x_scale = s.take(c.grad() ? 0 : pad * sizeof(float));
 	l.g = s.take(c.grad() ? (size_t)l.blocks * c.kw() * kBlockBytes : 0);
 	l.part = s.take((size_t)c.parts() * pad * sizeof(float2));
 	l.part_sum = s.take(c.ls != 0.0f ? (size_t)c.parts() * pad * sizeof(float) : 0);
@@ -327,9 +325,7 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 	float* row_loss = c.row_loss ? c.row_loss : m.at<float>(l.losses);
 	int* valid = m.at<int>(l.valid);
 	NNB_CUDA_TRY(cudaMemsetAsync(xr, 0, 2 * sizeof(split16::Range) + (size_t)c.P * sizeof(int), s));
-	// Where W and X are also a product's depth (the gradients) one scale serves the whole matrix, found in a
-	// pass of its own; for the loss alone every row has its own, found by the pack.
-	if (c.grad()) NNB_TRY(split16::find_ranges(s, c.x, c.P * c.D, c.w, c.V * c.D, xr));
+	NNB_TRY(split16::find_ranges(s, c.x, c.P * c.D, c.w, c.V * c.D, xr));
 	split16::Pack W, X, G;
 	W.buf = m.at<void>(l.wpack); W.rows = c.V; W.cols = c.D;
 	const long long rg = c.P / c.groups;             // parameter gradients are kept per group of rows
@@ -339,25 +335,13 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 			const int first = r0 == z * rg;
 			const float* x = c.x + r0 * c.D;
 			int* x_bad = m.at<int>(l.x_bad) + r0;
-			const long long w_blocks = (c.V + 2 * kRows - 1) / (2 * kRows) * 2;
-			const int count = r0 == 0 ? 2 : 1;               // W with the first piece
-			if (c.grad()) {
-				const split16::PackJob jobs[2] = {{x, n, c.D, blocks, xr, m.at<void>(l.xpack), x_bad},
-					{c.w, c.V, c.D, w_blocks, wr, m.at<void>(l.wpack), nullptr}};
-				NNB_TRY(split16::pack(s, jobs, count, parts));
-			} else {
-				const split16::RowPackJob jobs[2] = {{x, n, c.D, blocks, m.at<void>(l.xpack), m.at<float>(l.x_scale), x_bad, nullptr},
-					{c.w, c.V, c.D, w_blocks, m.at<void>(l.wpack), m.at<float>(l.w_scale), nullptr, &wr->bad}};
-				NNB_TRY(split16::pack_rows(s, jobs, count, parts));
-			}
+			const split16::PackJob jobs[2] = {{x, n, c.D, blocks, xr, m.at<void>(l.xpack), x_bad},
+				{c.w, c.V, c.D, (c.V + 2 * kRows - 1) / (2 * kRows) * 2, wr, m.at<void>(l.wpack), nullptr}};
+			NNB_TRY(split16::pack(s, jobs, r0 == 0 ? 2 : 1, parts));           // W with the first piece
 			X.buf = m.at<void>(l.xpack); X.rows = n; X.cols = c.D;
 
 			split16::Product p;
-			if (c.grad()) {
-				p.ra = xr; p.rb = wr;
-			} else {
-				p.row_scale = m.at<float>(l.x_scale); p.col_scale = m.at<float>(l.w_scale);
-			}
+			p.ra = xr; p.rb = wr;
 			p.bias = c.bias;
 			p.targets = c.targets + r0;
 			p.part = m.at<float2>(l.part);

@@ -139,69 +139,6 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
 	}
 }
 
-struct RowPackJobs {
-	RowPackJob job[2];
-	int vec[2], parts;
-};
-
-// A warp per row: its largest magnitude, then (from L1) its parts. grid.y: the matrix.
-__global__ void __launch_bounds__(256) pack_rows_kernel(const RowPackJobs jobs) {
-	const RowPackJob& w = jobs.job[blockIdx.y];
-	const int vec = jobs.vec[blockIdx.y], lane = threadIdx.x & 31;
-	const long long kw = (w.cols + kCols - 1) / kCols, quads = kw * (kCols / 4), rows = w.row_blocks * kRows;
-	chain_wait();
-	auto load = [&](long long r, long long q) {
-		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-		if (q * 4 >= w.cols) return v;
-		const float* src = w.x + r * w.cols + q * 4;
-		if (vec) return __ldg(reinterpret_cast<const float4*>(src));
-		v.x = __ldg(src);
-		if (q * 4 + 1 < w.cols) v.y = __ldg(src + 1);
-		if (q * 4 + 2 < w.cols) v.z = __ldg(src + 2);
-		if (q * 4 + 3 < w.cols) v.w = __ldg(src + 3);
-		return v;
-	};
-	for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
-		unsigned top = 0, bad = 0;
-		if (r < w.rows)
-#pragma unroll 4
-			for (long long q = lane; q < quads; q += 32) {
-				const float4 v = load(r, q);
-				for (float f : {v.x, v.y, v.z, v.w}) {
-					const unsigned b = __float_as_uint(f) & 0x7fffffffu;
-					if (b >= 0x7f800000u) bad = 1;
-					else top = max(top, b);
-				}
-			}
-		const Range range = {__reduce_max_sync(0xffffffffu, top), __reduce_or_sync(0xffffffffu, bad)};
-		const int shift = range_shift(&range);
-		const float s = exp2_int(shift);
-		if (lane == 0) {
-			w.scale[r] = exp2_int(-shift);
-			if (range.bad && w.row_bad) w.row_bad[r] = 1;
-			if (range.bad && w.bad) atomicOr(w.bad, 1u);
-		}
-		unsigned char* dst = static_cast<unsigned char*>(w.buf) + (r >> 7) * kw * kBlockBytes + (r & 127) * (kCols * 2);
-#pragma unroll 4
-		for (long long q = lane; q < quads; q += 32) {
-			float4 v = r < w.rows ? load(r, q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-			v.x = isfinite(v.x) ? v.x * s : 0.0f;
-			v.y = isfinite(v.y) ? v.y * s : 0.0f;
-			v.z = isfinite(v.z) ? v.z * s : 0.0f;
-			v.w = isfinite(v.w) ? v.w * s : 0.0f;
-			unsigned char* d = dst + (q >> 4) * kBlockBytes + (q & 15) * 8;
-			const uint2 hi = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
-			*reinterpret_cast<uint2*>(d) = hi;
-			if (jobs.parts == 2) {
-				const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)),
-					b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-				*reinterpret_cast<uint2*>(d + kPartBytes) = make_uint2(half2_bits(v.x - a.x, v.y - a.y),
-					half2_bits(v.z - b.x, v.w - b.y));
-			}
-		}
-	}
-}
-
 // ---- tcgen05 kind::f16 -----------------------------------------------------------------------
 
 // Instruction descriptor: fp32 accumulator, fp16 A and B.
@@ -454,19 +391,6 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 				}
 				__syncwarp();
 			};
-			if (kEpi == kStats && p.row_scale) {
-				// scales of this row and, through the staging tile, of the warp's 128 columns
-				const float rs = p.row_scale[gm];
-				st4[lane] = *reinterpret_cast<const float4*>(p.col_scale + n0 + 4 * lane);   // padded to whole tiles
-				__syncwarp();
-#pragma unroll
-				for (int j = 0; j < kBN / 8; ++j) {
-					const float4 cj = st4[j];
-					acc[2 * j] = mul2_rn(mul2_rn(acc[2 * j], make_float2(rs, rs)), make_float2(cj.x, cj.y));
-					acc[2 * j + 1] = mul2_rn(mul2_rn(acc[2 * j + 1], make_float2(rs, rs)), make_float2(cj.z, cj.w));
-				}
-				__syncwarp();
-			}
 			if (alpha2 != 1.0f) {
 #pragma unroll
 				for (int j = 0; j < kBN / 4; ++j) acc[j] = mul2_rn(acc[j], make_float2(alpha2, alpha2));
@@ -689,23 +613,6 @@ nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts) {
 		TraceScope ts(s, kTracePack);
 		NNB_CUDA_TRY(launch_chained(pack_kernel, dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 32), (unsigned)count),
 			256, 0, s, k));
-	}
-	return NNB_OK;
-}
-
-nnb_status pack_rows(cudaStream_t s, const RowPackJob* jobs, int count, int parts) {
-	RowPackJobs k;
-	k.parts = parts;
-	long long most = 0;
-	for (int i = 0; i < count; ++i) {
-		k.job[i] = jobs[i];
-		k.vec[i] = jobs[i].cols % 4 == 0 && (reinterpret_cast<uintptr_t>(jobs[i].x) & 15) == 0;
-		most = std::max(most, jobs[i].row_blocks * kRows);
-	}
-	{
-		TraceScope ts(s, kTracePack);
-		NNB_CUDA_TRY(launch_chained(pack_rows_kernel, dim3((unsigned)std::min<long long>((most + 7) / 8, 148 * 32),
-			(unsigned)count), 256, 0, s, k));
 	}
 	return NNB_OK;
 }
