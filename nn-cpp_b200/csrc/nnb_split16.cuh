@@ -90,8 +90,9 @@ struct Product {
 	int* err = nullptr;
 };
 
-// Ranges of x0[n0] and x1[n1] into out[0] and out[1], which the caller has zeroed.
-nnb_status find_ranges(cudaStream_t s, const float* x0, long long n0, const float* x1, long long n1, Range* out);
+// Ranges of the `groups` runs of n values of x into out[0 .. groups), and of w[nw] into out[groups]; the caller
+// has zeroed them.
+nnb_status find_ranges(cudaStream_t s, const float* x, long long n, long long groups, const float* w, long long nw, Range* out);
 
 // A matrix to pack: x [rows x cols] (row-major, dense) into buf, rows padded with zeros to `row_blocks` blocks;
 // values that are not finite become zero and set row_bad[row] (nullable, zeroed by the caller).

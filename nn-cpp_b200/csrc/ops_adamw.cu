@@ -367,6 +367,7 @@ void launch(cudaStream_t s, unsigned chunks, const List8<kCap>& l) {
 // Fills lists of up to kCap non-empty tensors (and 2^31 - 1 chunks) and launches each.
 template <typename List, int kCap>
 nnb_status run_lists(cudaStream_t s, const Scalars& sc, const Spec& a) {
+	DeviceState* dev = nullptr;
 	size_t i = 0;
 	while (i < a.count) {
 		List l;
@@ -388,6 +389,7 @@ nnb_status run_lists(cudaStream_t s, const Scalars& sc, const Spec& a) {
 		if (k == 0) return NNB_OK;                // only empty tensors were left
 		l.first[k] = (unsigned)chunks;
 		l.count = k;
+		NNB_TRY(device_state(&dev));
 		{
 			TraceScope ts(s, kTraceRowwise);
 			launch(s, (unsigned)chunks, l);

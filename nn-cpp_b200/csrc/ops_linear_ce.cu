@@ -301,8 +301,10 @@ Layout plan(const Call& c, Scratch& s) {
 	const size_t pad = (size_t)l.blocks * kRows;
 	l.dx_splits = c.dx ? split16::choose_splits(l.piece, c.D, c.V) : 1;
 	l.dw_splits = c.dw ? split16::choose_splits(c.V, c.D, l.piece) : 1;
-	l.ranges = s.take(2 * sizeof(split16::Range) + (size_t)c.P * sizeof(int));      // and x_bad: zeroed together
-	l.x_bad = l.ranges + 2 * sizeof(split16::Range);
+	// a range per group of x (a group's results depend on its own rows only) and w's, and x_bad: zeroed together
+	const size_t ranges = (size_t)(c.groups + 1) * sizeof(split16::Range);
+	l.ranges = s.take(ranges + (size_t)c.P * sizeof(int));
+	l.x_bad = l.ranges + ranges;
 	l.wpack = s.take(split16::pack_bytes(c.V, c.D));
 	l.xpack = s.take(split16::pack_bytes(l.piece, c.D));
 	l.g = s.take(c.grad() ? (size_t)l.blocks * c.kw() * kBlockBytes : 0);
@@ -320,19 +322,20 @@ Layout plan(const Call& c, Scratch& s) {
 
 nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l, const Scratch& m) {
 	const int parts = math_mode() == NNB_MATH_FP32X3 ? 2 : 1;
-	split16::Range* xr = m.at<split16::Range>(l.ranges);
-	split16::Range* wr = xr + 1;
+	split16::Range* ranges = m.at<split16::Range>(l.ranges);
+	const split16::Range* wr = ranges + c.groups;
 	float* row_loss = c.row_loss ? c.row_loss : m.at<float>(l.losses);
 	int* valid = m.at<int>(l.valid);
-	NNB_CUDA_TRY(cudaMemsetAsync(xr, 0, 2 * sizeof(split16::Range) + (size_t)c.P * sizeof(int), s));
-	NNB_TRY(split16::find_ranges(s, c.x, c.P * c.D, c.w, c.V * c.D, xr));
+	const long long rg = c.P / c.groups;             // parameter gradients are kept per group of rows
+	NNB_CUDA_TRY(cudaMemsetAsync(ranges, 0, (size_t)(c.groups + 1) * sizeof(split16::Range) + (size_t)c.P * sizeof(int), s));
+	NNB_TRY(split16::find_ranges(s, c.x, rg * c.D, c.groups, c.w, c.V * c.D, ranges));
 	split16::Pack W, X, G;
 	W.buf = m.at<void>(l.wpack); W.rows = c.V; W.cols = c.D;
-	const long long rg = c.P / c.groups;             // parameter gradients are kept per group of rows
 	for (long long z = 0; z < c.groups; ++z) {
 		for (long long r0 = z * rg; r0 < (z + 1) * rg;) {
 			const long long n = std::min(l.piece, (z + 1) * rg - r0), blocks = (n + kRows - 1) / kRows, pad = blocks * kRows;
 			const int first = r0 == z * rg;
+			const split16::Range* xr = ranges + z;
 			const float* x = c.x + r0 * c.D;
 			int* x_bad = m.at<int>(l.x_bad) + r0;
 			const split16::PackJob jobs[2] = {{x, n, c.D, blocks, xr, m.at<void>(l.xpack), x_bad},
@@ -411,6 +414,7 @@ nnb_status nnb_linear_ce_fwd(void* stream, size_t P, size_t D, size_t V, size_t 
 	const char* who = "linear_ce_fwd";
 	if (P == 0 || V == 0 || D == 0) return fail(NNB_ERR_SHAPE, "%s: empty input or weight", who);
 	if (groups == 0 || P % groups != 0) return fail(NNB_ERR_SHAPE, "%s: %zu rows in %zu groups", who, P, groups);
+	if (groups > 65534) return fail(NNB_ERR_UNSUPPORTED, "%s: more than 65534 groups", who);
 	if (!(label_smoothing >= 0.0f && label_smoothing < 1.0f))
 		return fail(NNB_ERR_INVALID, "%s: label_smoothing must be in [0, 1)", who);
 	if (!x || !w || !targets || !loss || !norm) return fail(NNB_ERR_INVALID, "%s: null pointer", who);

@@ -276,6 +276,8 @@ nnb_status nnb_residual_norm_fwd(void* stream, size_t R, size_t D, size_t gate_r
 	if (!x || !y || (!branch) != (!h)) return fail(NNB_ERR_INVALID, "residual_norm_fwd: null pointer");
 	if (!branch && (gate || post_gamma)) return fail(NNB_ERR_INVALID, "residual_norm_fwd: a gate or post_gamma without a branch");
 	if (reinterpret_cast<uintptr_t>(stats) & 15) return fail(NNB_ERR_INVALID, "residual_norm_fwd: stats must be 16-byte aligned");
+	DeviceState* dev = nullptr;
+	NNB_TRY(device_state(&dev));
 	Row p;
 	p.x = x; p.branch = branch; p.post_gamma = post_gamma; p.post_beta = post_beta; p.gate = gate;
 	p.gamma = gamma; p.beta = beta; p.h = h; p.y = y; p.stats = reinterpret_cast<float4*>(stats);
@@ -323,6 +325,8 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 	const bool needs_branch = gate || post_gamma;
 	if (!stats || (!dh && !dy) || (dy && !h) || (needs_branch && !branch)) return fail(NNB_ERR_INVALID, "%s: null pointer", who);
 	if (reinterpret_cast<uintptr_t>(stats) & 15) return fail(NNB_ERR_INVALID, "%s: stats must be 16-byte aligned", who);
+	DeviceState* dev = nullptr;
+	NNB_TRY(device_state(&dev));
 	Grad p;
 	p.dh = dh; p.dy = dy; p.h = h; p.branch = branch; p.post_gamma = post_gamma; p.post_beta = post_beta;
 	p.gate = gate; p.gamma = gamma; p.stats = reinterpret_cast<const float4*>(stats);

@@ -25,17 +25,18 @@ namespace {
 // ---- range and pack --------------------------------------------------------------------------
 
 struct RangeJobs {
-	const float* x[2];
-	long long n[2];
-	int vec[2];
+	const float *x, *w;
+	long long n, nw;                           // of each group of x, and of w
+	int vec, vec_w, groups;
 	Range* out;
 };
 
-// grid.y: the matrix.
+// grid.y: the groups of x, then w.
 __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
-	const float* __restrict__ x = jobs.x[blockIdx.y];
-	const long long n = jobs.n[blockIdx.y];
-	const int vec = jobs.vec[blockIdx.y];
+	const bool is_w = (int)blockIdx.y == jobs.groups;
+	const float* __restrict__ x = is_w ? jobs.w : jobs.x + blockIdx.y * jobs.n;
+	const long long n = is_w ? jobs.nw : jobs.n;
+	const int vec = is_w ? jobs.vec_w : jobs.vec;
 	Range* out = jobs.out + blockIdx.y;
 	chain_wait();
 	unsigned top = 0, bad = 0;
@@ -577,21 +578,16 @@ nnb_status dispatch(cudaStream_t s, const DeviceState* dev, int epilogue, bool m
 
 }  // namespace
 
-nnb_status find_ranges(cudaStream_t s, const float* x0, long long n0, const float* x1, long long n1, Range* out) {
+nnb_status find_ranges(cudaStream_t s, const float* x, long long n, long long groups, const float* w, long long nw, Range* out) {
 	RangeJobs jobs;
-	const float* xs[2] = {x0, x1};
-	const long long ns[2] = {n0, n1};
-	for (int i = 0; i < 2; ++i) {
-		jobs.x[i] = xs[i];
-		jobs.n[i] = ns[i];
-		jobs.vec[i] = ns[i] % 4 == 0 && (reinterpret_cast<uintptr_t>(xs[i]) & 15) == 0;
-	}
-	jobs.out = out;
-	const long long n = std::max(n0, n1);
+	jobs.x = x; jobs.n = n; jobs.groups = (int)groups; jobs.w = w; jobs.nw = nw; jobs.out = out;
+	jobs.vec = n % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+	jobs.vec_w = nw % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+	const long long most = std::max(n, nw);
 	{
 		TraceScope ts(s, kTracePack);
-		NNB_CUDA_TRY(launch_chained(range_kernel, dim3((unsigned)std::min<long long>((n + 4095) / 4096, 148 * 8), 2), 256, 0, s,
-			jobs));
+		NNB_CUDA_TRY(launch_chained(range_kernel, dim3((unsigned)std::min<long long>((most + 4095) / 4096, 148 * 8),
+			(unsigned)(groups + 1)), 256, 0, s, jobs));
 	}
 	return NNB_OK;
 }

@@ -541,7 +541,8 @@ class AdamW:
     (nnb_adamw8_multi_step, include/nnb.h): 2 bytes of state per parameter instead of 8.
 
     The states are one flat buffer each, flat_m and flat_v, parameter i's part starting at offsets[i]
-    (a whole number of 256-element blocks) with zeros behind it; m[i] and v[i] are views of the parts.
+    (a whole number of 256-element blocks) with zeros behind it; m[i] and v[i] are views of the parts (to be
+    filled, not replaced).
     With 8 bits they hold the codes, and unit_m / unit_v the units, block after block."""
 
     BLOCK = 256
@@ -570,7 +571,7 @@ class AdamW:
 
         kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
         self.flat_m, self.flat_v = (zeros(total, k) for k in kinds)
-        self.m, self.v = ([flat[o: o + n].view(p.data.shape) for p, n, o in zip(self.params, sizes, self.offsets)]
+        self.m, self.v = (tuple(flat[o: o + n].view(p.data.shape) for p, n, o in zip(self.params, sizes, self.offsets))
                           for flat in (self.flat_m, self.flat_v))
         self._sizes, self._n = sizes, (ctypes.c_size_t * len(sizes))(*sizes)
         self._states = [_pointers([t.data_ptr() for t in ts]) for ts in (self.m, self.v)]

@@ -258,6 +258,34 @@ def test_parameter_groups(cuda):
         assert torch.equal(vals["w"].grad[z].view(V, D), part["w"]) and torch.equal(vals["b"].grad[z], part["b"])
 
 
+def test_groups_of_different_size(cuda):
+    """A group's bits are its own whatever the other groups hold: here one 2^30 times larger, next to values
+    that its scale would have lost."""
+    G, P, D, V = 2, 2 * 32, 24, 50
+    x, w, b, t = _make(P, D, V, seed=17)
+    x[:32] *= 2.0 ** 30
+    x[32:, ::3] *= 2.0 ** -12
+    vals = {"x": Value.leaf(x, True), "w": Value.leaf(w, True), "b": Value.leaf(b, True)}
+    for k, n in (("w", V * D), ("b", V)):
+        vals[k].grad, vals[k].grad_fresh = torch.empty(G, n, device="cuda"), True
+    norm = torch.tensor([1.0 / 32], device="cuda")
+    with F.param_groups(G):
+        F.linear_cross_entropy(vals["x"], vals["w"], vals["b"], t, grad_norm=norm).backward()
+    _, part = _run(x[32:].contiguous(), w, b, t[32:].contiguous(), grad_norm=norm)
+    assert torch.equal(vals["x"].grad[32:], part["x"])
+    assert torch.equal(vals["w"].grad[1].view(V, D), part["w"]) and torch.equal(vals["b"].grad[1], part["b"])
+
+
+def test_ignored_rows_may_hold_anything(cuda):
+    x, w, b, t = _make(40, 32, 64, seed=18)
+    t[7], t[20] = IGNORE, IGNORE
+    want = _run(x, w, b, t)
+    x2 = x.clone()
+    x2[7], x2[20] = math.nan, math.inf
+    got = _run(x2, w, b, t)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(got[1][k], want[1][k]) for k in want[1])
+
+
 def test_tf32_mode(cuda):
     """The fast mode: operands of 11 significant bits, 2^-11 of each term's two factors."""
     x, w, b, t = _make(300, 64, 500, seed=11)
