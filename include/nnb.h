@@ -231,8 +231,9 @@ NNB_API nnb_status nnb_layernorm_bwd_grouped(void* stream, size_t R, size_t D, s
  *   p = branch, or norm(branch; post_gamma, post_beta) when post_gamma is not NULL
  *   h = x + scale * gate * p          gate NULL: 1
  *   y = norm(h; gamma, beta)
- * over R rows of D values (D <= 16384). branch and h NULL: y = norm(x) alone. kind NNB_NORM_LAYER: (a - mean) / sqrt(var + eps) * gamma + beta;
- * NNB_NORM_RMS: a / sqrt(mean a^2 + eps) * gamma, beta and post_beta NULL. gate holds gate_rows rows of D,
+ * over R rows of D values (D <= 16384). branch and h NULL: y = norm(x) alone. kind NNB_NORM_LAYER:
+ * (a - mean) / sqrt(var + eps) * gamma + beta; NNB_NORM_RMS: a / sqrt(mean a^2 + eps) * gamma, beta and
+ * post_beta NULL. gate holds gate_rows rows of D,
  * each serving R / gate_rows consecutive rows (1: a parameter per channel; ignored when gate is NULL).
  * stats (R rows of 4 floats, 16-byte aligned; NULL: not kept) is what the backward needs. No other buffer
  * has an alignment rule; 16 bytes and D % 4 == 0 run fastest. */
@@ -249,15 +250,14 @@ typedef struct nnb_grad_out {
 } nnb_grad_out;
 /* Gradients of nnb_residual_norm_fwd from dh and dy (either may be NULL: zeros), the forward's h and
  * stats, and its operands (branch may be NULL without post_gamma and gate; after a forward without a
- * branch h is x). Each nnb_grad_out may be
- * NULL. dx also receives what reaches h through y. Parameter gradients (a gate of one row included) are
- * kept per group of R / groups consecutive rows, as nnb_layernorm_bwd_grouped's; a gate of several rows
- * needs gate_rows % groups == 0. The sums' order depends on D, R / groups and the gate's span only. */
+ * branch h is x). grads: seven outputs in the order dx, dbranch, dpost_gamma, dpost_beta, dgate, dgamma,
+ * dbeta (a host array, read before the call returns). dx also receives what reaches h through y.
+ * Parameter gradients (a gate of one row included) are kept per group of R / groups consecutive rows, as
+ * nnb_layernorm_bwd_grouped's; a gate of several rows needs gate_rows % groups == 0. The sums' order
+ * depends on D, R / groups and the gate's span only. */
 NNB_API nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups, size_t gate_rows, int kind,
 		float scale, const float* dh, const float* dy, const float* h, const float* branch, const float* post_gamma,
-		const float* post_beta, const float* gate, const float* gamma, const float* stats, const nnb_grad_out* dx,
-		const nnb_grad_out* dbranch, const nnb_grad_out* dpost_gamma, const nnb_grad_out* dpost_beta,
-		const nnb_grad_out* dgate, const nnb_grad_out* dgamma, const nnb_grad_out* dbeta);
+		const float* post_beta, const float* gate, const float* gamma, const float* stats, const nnb_grad_out* grads);
 /* Training-mode batchnorm over [N, C, S] (ops.hpp:114; ops.cpp:900-961): per-channel statistics with
  * the reference's fp64 sums of 8-lane partials; fuse_relu folds a ReLU and writes its 1-byte alive
  * mask; mean, var (biased) and inv_std (C each) are written. */

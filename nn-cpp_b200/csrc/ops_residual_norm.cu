@@ -292,9 +292,7 @@ nnb_status nnb_residual_norm_fwd(void* stream, size_t R, size_t D, size_t gate_r
 
 nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups, size_t gate_rows, int kind, float scale,
 		const float* dh, const float* dy, const float* h, const float* branch, const float* post_gamma,
-		const float* post_beta, const float* gate, const float* gamma, const float* stats, const nnb_grad_out* dx,
-		const nnb_grad_out* dbranch, const nnb_grad_out* dpost_gamma, const nnb_grad_out* dpost_beta,
-		const nnb_grad_out* dgate, const nnb_grad_out* dgamma, const nnb_grad_out* dbeta) {
+		const float* post_beta, const float* gate, const float* gamma, const float* stats, const nnb_grad_out* grads) {
 	using namespace nnb;
 	const char* who = "residual_norm_bwd";
 	NNB_TRY(check_common(who, R, D, gate_rows, kind, gate, post_gamma != nullptr, post_beta, gamma, nullptr, false));
@@ -303,24 +301,22 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 	const bool gate_param = gate && gate_rows == 1;
 	if (gate && !gate_param && gate_rows % groups != 0)
 		return fail(NNB_ERR_SHAPE, "%s: %zu gate rows in %zu groups", who, gate_rows, groups);
-	static const nnb_grad_out none = {nullptr, 0, 1};
-	auto pick = [](const nnb_grad_out* g) { return g ? *g : none; };
-	const nnb_grad_out gx = pick(dx), gb = pick(dbranch), gg = pick(dgate);
-	if ((kind == NNB_NORM_RMS && (pick(dbeta).p || pick(dpost_beta).p)) || (!post_gamma && (pick(dpost_gamma).p ||
-			pick(dpost_beta).p)) || (!gate && gg.p))
+	if (!grads) return fail(NNB_ERR_INVALID, "%s: null pointer", who);
+	const nnb_grad_out &gx = grads[0], &gb = grads[1], &gg = grads[4];
+	// the parameters' sums, in the kernel's order
+	const nnb_grad_out outs[kArrays] = {grads[5], grads[6], grads[2], grads[3], gate_param ? gg : nnb_grad_out{nullptr, 0, 1}};
+	if ((kind == NNB_NORM_RMS && (outs[1].p || outs[3].p)) || (!post_gamma && (outs[2].p || outs[3].p)) || (!gate && gg.p))
 		return fail(NNB_ERR_INVALID, "%s: a gradient of a parameter that is not there", who);
-	for (const nnb_grad_out* g : {dpost_gamma, dpost_beta, dgamma, dbeta, gate_param ? dgate : nullptr})
-		if (g && g->p && g->stride && g->stride < D && groups > 1)
+	for (int i = 0; i < kArrays; ++i) {
+		if (outs[i].p && outs[i].stride && outs[i].stride < D && groups > 1)
 			return fail(NNB_ERR_INVALID, "%s: the groups' gradients overlap", who);
-	const float* sums[kArrays] = {pick(dgamma).p, pick(dbeta).p, pick(dpost_gamma).p, pick(dpost_beta).p,
-		gate_param ? gg.p : nullptr};
-	for (int i = 0; i < kArrays; ++i)
 		for (int j = 0; j < i; ++j)
-			if (sums[i] && sums[i] == sums[j]) return fail(NNB_ERR_INVALID, "%s: two parameters share a gradient buffer", who);
+			if (outs[i].p && outs[i].p == outs[j].p)
+				return fail(NNB_ERR_INVALID, "%s: two parameters share a gradient buffer", who);
+	}
 	cudaStream_t s = static_cast<cudaStream_t>(stream);
 	if (R == 0) {
-		for (const nnb_grad_out* g : {dpost_gamma, dpost_beta, dgamma, dbeta, gate_param ? dgate : nullptr})
-			NNB_TRY(zero_rows(s, pick(g), groups, D));
+		for (const nnb_grad_out& g : outs) NNB_TRY(zero_rows(s, g, groups, D));
 		return gate_param || !gate ? NNB_OK : zero_rows(s, nnb_grad_out{gg.p, D, gg.first}, gate_rows, D);
 	}
 	const bool needs_branch = gate || post_gamma;
@@ -372,7 +368,6 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 			: (post_gamma ? bwd_scalar_post : bwd_scalar)(s, p, (long long)groups);
 	}
 	Outs o;
-	const nnb_grad_out outs[kArrays] = {pick(dgamma), pick(dbeta), pick(dpost_gamma), pick(dpost_beta), gate_param ? gg : none};
 	bool any = false;
 	int arrays = 0;
 	for (int i = 0; i < kArrays; ++i) {

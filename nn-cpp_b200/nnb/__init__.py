@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import pathlib
 import re
+import struct
 
 _PKG = pathlib.Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libnnb.so"
@@ -132,8 +133,7 @@ _SIGS = {
     "nnb_adamw8_multi_step": ([_p, _sz, _p, _p, _p, _p, _p, _p, _p, _f, _f, _f, _f, _f, _c.c_longlong], _i),
     "nnb_adamw8_moments": ([_p, _sz, _p, _p, _p, _p, _p, _p], _i),
     "nnb_residual_norm_fwd": ([_p, _sz, _sz, _sz, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p], _i),
-    "nnb_residual_norm_bwd": ([_p, _sz, _sz, _sz, _sz, _i, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
-                               _p], _i),
+    "nnb_residual_norm_bwd": ([_p, _sz, _sz, _sz, _sz, _i, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p], _i),
     "nnb_linear_ce_fwd": ([_p, _sz, _sz, _sz, _sz, _p, _p, _p, _p, _c.c_int64, _f, _p, _p, _p, _p, _p, _sz, _p, _sz], _i),
     "nnb_scaled_accumulate": ([_p, _sz, _p, _p, _p], _i),
     "nnb_manual_seed": ([_c.c_uint64], None),
@@ -156,9 +156,12 @@ _SIGS = {
 }
 
 
-class GradOut(_c.Structure):
-    """nnb_grad_out: a gradient output of nnb_residual_norm_bwd."""
-    _fields_ = [("p", _p), ("stride", _sz), ("first", _i)]
+_GRAD_OUTS = struct.Struct("PNi" * 7 + "0P")
+
+
+def grad_outs(*outs) -> bytes:
+    """The seven nnb_grad_out of nnb_residual_norm_bwd from (address or None, stride, first) or None each."""
+    return _GRAD_OUTS.pack(*(f for o in outs for f in ((o[0] or 0, o[1], o[2]) if o is not None else (0, 0, 1))))
 
 
 class ScaledGrad(_c.Structure):

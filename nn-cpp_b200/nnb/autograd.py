@@ -124,11 +124,13 @@ def backward(roots: Sequence[Value], seeds: Sequence[torch.Tensor | None]) -> No
     if len({id(r) for r in roots}) != len(roots):
         raise ValueError("backward(): the same root twice")
     for root, seed in zip(roots, seeds):
-        if seed is None and root.data.numel() != 1:
-            raise ValueError("backward() needs a single-element value (AutogradShapeError)")
-        if seed is not None and seed.numel() != root.data.numel():
+        data = root.data
+        if seed is None:
+            if data.numel() != 1:
+                raise ValueError("backward() needs a single-element value (AutogradShapeError)")
+        elif seed.numel() != data.numel():
             raise ValueError("backward(): the seed must have the root's element count")
-        if seed is not None and (seed.dtype is not root.data.dtype or seed.device != root.data.device):
+        elif seed.dtype is not data.dtype or seed.get_device() != data.get_device():
             raise ValueError("backward(): the seed must have the root's type and device")
     # iterative post-order walk over the values that have a rule (a value without one has no parents)
     topo: list[Value] = []

@@ -15,7 +15,7 @@ import weakref
 
 import torch
 
-from . import NORM_LAYER, NORM_RMS, GradOut, ScaledGrad, TensorShapeError, check, lib
+from . import NORM_LAYER, NORM_RMS, ScaledGrad, TensorShapeError, check, grad_outs, lib
 from .autograd import Value, current_stream as _s, empty
 
 
@@ -411,12 +411,13 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
             if v is None or not _need(v):
                 return None
             buf, first = v.grad_accum()
-            return ctypes.byref(GradOut(buf.data_ptr(), _gstride(buf, v) if grouped else 0, first))
+            return buf.data_ptr(), _gstride(buf, v) if grouped else 0, first
+        norm = (out(gamma, True), out(beta, True)) if dy is not None else (None, None)
+        grads = grad_outs(out(x, False), out(branch, False), out(post_gamma, True), out(post_beta, True),
+                          out(gate, gate_rows == 1), *norm)
         check(lib().nnb_residual_norm_bwd(_s(), R, D, _GROUPS, gate_rows, k, scale, _p(dh), _p(dy), _p(h_data),
                                           _p(branch.data), opt(post_gamma), opt(post_beta), opt(gate), _p(gamma.data),
-                                          _p(stats), out(x, False), out(branch, False), out(post_gamma, True),
-                                          out(post_beta, True), out(gate, gate_rows == 1),
-                                          *((out(gamma, True), out(beta, True)) if dy is not None else (None, None))))
+                                          _p(stats), grads))
 
     def h_backward(g):
         dy = held.pop() if held else None
@@ -451,8 +452,9 @@ def rmsnorm(x: Value, gamma: Value, eps: float) -> Value:
         dx, fx = x.grad_accum() if _need(x) else (None, 0)
         dg, fg = gamma.grad_accum() if _need(gamma) else (None, 0)
         check(lib().nnb_residual_norm_bwd(_s(), R, D, _GROUPS, 0, NORM_RMS, 1.0, None, _p(g), _p(x.data), None, None, None,
-                                          None, _p(gamma.data), _p(stats), ctypes.byref(GradOut(_p(dx), 0, fx)), None, None,
-                                          None, None, ctypes.byref(GradOut(_p(dg), _gstride(dg, gamma), fg)), None))
+                                          None, _p(gamma.data), _p(stats),
+                                          grad_outs((_p(dx), 0, fx), None, None, None, None,
+                                                    (_p(dg), _gstride(dg, gamma), fg), None)))
 
     return Value.node(y, (x, gamma), backward)
 

@@ -1,11 +1,9 @@
 """Refusals of the residual norm (host checks only, no GPU needed)."""
-import ctypes
-
 import pytest
 import torch
 
 import nnb
-from nnb import GradOut, NORM_LAYER, NORM_RMS, TensorShapeError
+from nnb import NORM_LAYER, NORM_RMS, TensorShapeError, grad_outs
 from nnb import functional as F
 from nnb.autograd import Value, backward
 
@@ -20,10 +18,10 @@ def _fwd(R=4, D=8, gate_rows=0, kind=NORM_LAYER, x=P, branch=P, pg=None, pb=None
 
 def _bwd(R=4, D=8, groups=1, gate_rows=0, kind=NORM_LAYER, dh=P, dy=P, h=P, branch=P, pg=None, pb=None, gate=None, gamma=P,
          stats=P, outs=()):
-    outs = {k: ctypes.byref(GradOut(*v)) for k, v in dict(outs).items()}
+    outs = dict(outs)
     names = ("dx", "dbranch", "dpost_gamma", "dpost_beta", "dgate", "dgamma", "dbeta")
     return nnb.lib().nnb_residual_norm_bwd(None, R, D, groups, gate_rows, kind, 1.0, dh, dy, h, branch, pg, pb, gate, gamma,
-                                           stats, *[outs.get(n) for n in names])
+                                           stats, grad_outs(*[outs.get(n) for n in names]))
 
 
 def test_forward_refusals():

@@ -341,11 +341,9 @@ def test_rmsnorm(cuda, R, D):
 
 def test_no_rows(cuda):
     """The C entry with R == 0: stored parameter gradients become zeros, added ones stay."""
-    import ctypes
-
-    from nnb import GradOut, check, lib
+    from nnb import check, grad_outs, lib
     a, b = torch.ones(8, device="cuda"), torch.ones(8, device="cuda")
-    outs = [None, None, None, None, None, ctypes.byref(GradOut(a.data_ptr(), 0, 1)), ctypes.byref(GradOut(b.data_ptr(), 0, 0))]
+    outs = grad_outs(None, None, None, None, None, (a.data_ptr(), 0, 1), (b.data_ptr(), 0, 0))
     check(lib().nnb_residual_norm_bwd(torch.cuda.current_stream().cuda_stream, 0, 8, 1, 0, 0, 1.0, None, None, None, None,
-                                      None, None, None, a.data_ptr(), None, *outs))
+                                      None, None, None, a.data_ptr(), None, outs))
     assert torch.equal(a, torch.zeros(8, device="cuda")) and torch.equal(b, torch.ones(8, device="cuda"))
