@@ -14,6 +14,7 @@ torch provides allocation and streams only; every number is produced by a kernel
 from __future__ import annotations
 
 import functools
+import threading
 from typing import Callable, Sequence
 
 import torch
@@ -115,6 +116,19 @@ class Value:
         backward((self,), (seed,))
 
 
+class _Run(threading.local):
+    token: object = None
+
+
+_RUN = _Run()
+
+
+def running() -> object:
+    """A token of this thread's running backward pass: a rule that leaves something for a later rule of
+    the same pass keeps the token beside it, so that what a pass that failed half-way left is not used."""
+    return _RUN.token
+
+
 def backward(roots: Sequence[Value], seeds: Sequence[torch.Tensor | None]) -> None:
     """Value.backward from several roots at once, each with its upstream gradient (None: 1, for a
     single-element root): the gradients of the sum over roots of sum(root * seed). A root may depend on
@@ -160,6 +174,10 @@ def backward(roots: Sequence[Value], seeds: Sequence[torch.Tensor | None]) -> No
         seed = _one(root.data.device) if seed is None else seed.contiguous()
         root.grad = seed if seed.shape == root.data.shape else seed.view(root.data.shape)
         root.grad_fresh, root.grad_borrowed = False, True
-    for v in reversed(topo):
-        if v.backward_fn is not None:
-            v.backward_fn(v.grad)
+    outer, _RUN.token = _RUN.token, object()
+    try:
+        for v in reversed(topo):
+            if v.backward_fn is not None:
+                v.backward_fn(v.grad)
+    finally:
+        _RUN.token = outer

@@ -16,7 +16,7 @@ import weakref
 import torch
 
 from . import NORM_LAYER, NORM_RMS, ScaledGrad, TensorShapeError, check, grad_outs, lib
-from .autograd import Value, current_stream as _s, empty
+from .autograd import Value, current_stream as _s, empty, running
 
 
 def _p(t):
@@ -404,7 +404,7 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     check(lib().nnb_residual_norm_fwd(_s(), R, D, gate_rows, k, eps, scale, _p(x.data), _p(branch.data), opt(post_gamma),
                                       opt(post_beta), opt(gate), _p(gamma.data), opt(beta), _p(h_data), _p(y_data),
                                       _p(stats)))
-    held = []          # what reached y in the running backward
+    held = []          # (backward pass, what reached y in it)
 
     def run(dh, dy):
         def out(v, grouped):
@@ -420,13 +420,15 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
                                           _p(stats), grads))
 
     def h_backward(g):
-        dy = held.pop() if held else None
+        at, dy = held.pop() if held else (None, None)
+        if at is not running():
+            dy = None
         node = h_ref()
         run(None if node is not None and node.grad_fresh else g, dy)
 
     def y_backward(g):
         if h.requires_grad:
-            held[:] = [g]
+            held[:] = [(running(), g)]
         else:
             run(None, g)
 

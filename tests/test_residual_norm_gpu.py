@@ -347,3 +347,27 @@ def test_no_rows(cuda):
     check(lib().nnb_residual_norm_bwd(torch.cuda.current_stream().cuda_stream, 0, 8, 1, 0, 0, 1.0, None, None, None, None,
                                       None, None, None, a.data_ptr(), None, outs))
     assert torch.equal(a, torch.zeros(8, device="cuda")) and torch.equal(b, torch.ones(8, device="cuda"))
+
+
+def test_backward_after_one_that_failed(cuda):
+    """A pass that stops between y's rule and h's leaves nothing for the next pass, from h alone."""
+    def leaves():
+        g = torch.Generator(device="cuda").manual_seed(3)
+        return [Value(torch.randn(*s, generator=g, device="cuda"), True) for s in ((6, 16), (6, 16), (16,), (16,))]
+
+    def fail(_):
+        raise RuntimeError("a rule that fails")
+
+    seed = torch.ones(6, 16, device="cuda")
+    broken, fresh = leaves(), leaves()
+    h, y = F.residual_norm(*broken)
+    failing = Value.node(seed.clone(), (h,), fail)
+    with pytest.raises(RuntimeError, match="a rule that fails"):
+        backward((y, failing), (seed, seed))       # rules run in the order y, failing, h or failing, y, h
+    with pytest.raises(RuntimeError, match="a rule that fails"):
+        backward((failing, y), (seed, seed))
+    backward((h,), (seed,))
+    h, _ = F.residual_norm(*fresh)
+    backward((h,), (seed,))
+    for a, b in zip(broken[:2], fresh[:2]):
+        assert torch.equal(a.grad, b.grad)
