@@ -857,6 +857,12 @@ def _linear_ce_args(who: str, x, weight, bias, targets):
     return x.data.numel() // xs[-1], xs[-1], ws[0]
 
 
+def _check_grad_norm(grad_norm) -> None:
+    if grad_norm is not None and grad_norm.numel() != 1:
+        raise TensorShapeError("linear_cross_entropy: grad_norm must hold one value")
+    _check_buffers("linear_cross_entropy", (grad_norm,))
+
+
 def linear_cross_entropy(x: Value, weight: Value, bias: Value | None, targets: torch.Tensor, ignore_index: int = -100,
                          label_smoothing: float = 0.0, grad_norm: torch.Tensor | None = None) -> Value:
     """sequence_cross_entropy(linear(x, weight, bias), targets) without keeping the logits: x [..., D],
@@ -866,6 +872,7 @@ def linear_cross_entropy(x: Value, weight: Value, bias: Value | None, targets: t
     The rows go through in pieces; where a gradient is needed it is computed with the loss, from the same
     logits, and the backward only scales it (nnb_linear_ce_fwd, include/nnb.h). For inputs that need
     none, see linear_token_losses."""
+    _check_grad_norm(grad_norm)
     P, D, V = _linear_ce_args("linear_cross_entropy", x, weight, bias, targets)
     parents = (x, weight) if bias is None else (x, weight, bias)
     params = any(_need(v) for v in parents[1:])

@@ -54,3 +54,14 @@ def test_function_refusals(op):
             op(x, w, b, tt)
     with pytest.raises(ValueError, match="current CUDA device"):
         op(*good, t)
+
+
+def test_grad_norm_refusals():
+    v = lambda *s: Value(torch.zeros(s))      # noqa: E731
+    args = (v(2, 3, 8), v(5, 8), v(5), torch.zeros(2, 3, dtype=torch.int64))
+    assert F._check_grad_norm(None) is None
+    with pytest.raises(ValueError, match="current CUDA device"):
+        F._check_grad_norm(torch.ones(1))
+    for bad in (torch.ones(2), torch.ones(0)):
+        with pytest.raises(TensorShapeError, match="one value"):
+            F.linear_cross_entropy(*args, grad_norm=bad)
