@@ -337,7 +337,9 @@ __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t
 
 // A chained kernel's first step (launch_chained): lets the next kernel of the chain be launched as soon as
 // every CTA of this one has got here, then waits until the previous kernel has finished and its writes are
-// visible. Nothing before it may touch memory that an earlier kernel writes or reads.
+// visible. Nothing before it may touch memory that an earlier kernel writes or reads. What an earlier kernel of
+// the chain may have written is read with plain loads: __ldg and `const T* __restrict__` promise that the memory
+// does not change while the kernel lives, and such a load may be moved to before the wait.
 __device__ __forceinline__ void chain_wait() {
 	asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 	asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -87,15 +87,6 @@ struct Pack {
 	float v[VEC];
 	__device__ __forceinline__ void load(const float* p) {
 		if constexpr (VEC == 4) {
-			const float4 t = __ldg(reinterpret_cast<const float4*>(p));
-			v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-		} else {
-			v[0] = __ldg(p);
-		}
-	}
-	// plain load: the buffer is also written by this kernel
-	__device__ __forceinline__ void load_rw(const float* p) {
-		if constexpr (VEC == 4) {
 			const float4 t = *reinterpret_cast<const float4*>(p);
 			v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
 		} else {
@@ -127,7 +118,7 @@ __device__ __forceinline__ void store_grad(float* dst, Pack<VEC> v, int first) {
 		for (int i = 0; i < VEC; ++i) v.v[i] = v.v[i] + 0.0f;
 	} else {
 		Pack<VEC> o;
-		o.load_rw(dst);
+		o.load(dst);
 #pragma unroll
 		for (int i = 0; i < VEC; ++i) v.v[i] = o.v[i] + v.v[i];
 	}
@@ -219,11 +210,11 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 #pragma unroll
 		for (int u = 0; u < KV; ++u) {
 			dt[u].zero();
-			if (in[u] && with_dh) dt[u].load_rw(stage + u * kStep);
+			if (in[u] && with_dh) dt[u].load(stage + u * kStep);
 			if constexpr (kBranch) {
 				br[u].zero();
 				if constexpr (kStaged == 4) {
-					if (in[u]) br[u].load_rw(stage + 3 * D + u * kStep);
+					if (in[u]) br[u].load(stage + 3 * D + u * kStep);
 				} else {
 					if (in[u]) br[u].load(p.branch + off + u * kStep);
 				}
@@ -237,8 +228,8 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 				g.zero();
 				hat[u].zero();
 				if (in[u]) {
-					dy.load_rw(stage + D + u * kStep);
-					hat[u].load_rw(stage + 2 * D + u * kStep);
+					dy.load(stage + D + u * kStep);
+					hat[u].load(stage + 2 * D + u * kStep);
 					g.load(p.gamma + j0 + u * kStep);
 				}
 #pragma unroll

@@ -45,10 +45,10 @@ struct RowInfo {
 
 // A row's statistics from its parts (eight rows per CTA, 32 threads to a row: few rows must fill the GPU), its
 // loss and RowInfo.
-__global__ void __launch_bounds__(256) ce_rows_kernel(const float2* __restrict__ part, const float* __restrict__ part_sum,
-		const float* __restrict__ target_logit, int parts, int rows, int rows_pad, int V, const int64_t* __restrict__ targets,
-		int64_t ignore_index, float ls, const int* __restrict__ x_bad, const split16::Range* __restrict__ w_range,
-		float* __restrict__ row_loss, int* __restrict__ valid, RowInfo* __restrict__ info, int* err) {
+__global__ void __launch_bounds__(256) ce_rows_kernel(const float2* part, const float* part_sum,
+		const float* target_logit, int parts, int rows, int rows_pad, int V, const int64_t* targets,
+		int64_t ignore_index, float ls, const int* x_bad, const split16::Range* w_range,
+		float* row_loss, int* valid, RowInfo* info, int* err) {
 	__shared__ float2 ms[32][9];
 	__shared__ float tot[32][9];
 	const int x = threadIdx.x & 7, y = threadIdx.x >> 3, r = blockIdx.x * 8 + x;
@@ -108,8 +108,8 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // One block of 128 rows x 64 columns per CTA, in place: logits in, G out as fp16 parts; its column sums.
 // A thread holds four columns of eight rows. HBM bound: 4 bytes in and 4 out per logit (185 us for 134 M
 // logits, 5.8 TB/s).
-__global__ void __launch_bounds__(256) ce_grad_kernel(float* __restrict__ blocks, int kw, int V, int rows_pad,
-		const RowInfo* __restrict__ info, float ls, int two_parts, float* __restrict__ col_part) {
+__global__ void __launch_bounds__(256) ce_grad_kernel(float* blocks, int kw, int V, int rows_pad,
+		const RowInfo* info, float ls, int two_parts, float* col_part) {
 	__shared__ float4 sums[8][16];
 	const int c64 = blockIdx.x, rb = blockIdx.y, tid = threadIdx.x, q = tid & 15, r0 = tid >> 4;
 	float* block = blocks + ((long long)rb * kw + c64) * (kRows * kCols);
@@ -172,15 +172,15 @@ __global__ void __launch_bounds__(256) ce_grad_kernel(float* __restrict__ blocks
 
 // db (+)= the row blocks' column sums: 32 columns per CTA, warp y sums blocks y, y + 8, ..., then the eight
 // sums in order.
-__global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ col_part, int row_blocks, int ld, int V,
-		float* __restrict__ db, int first) {
+__global__ void __launch_bounds__(256) ce_bias_kernel(const float* col_part, int row_blocks, int ld, int V,
+		float* db, int first) {
 	__shared__ float tile[8][32];
 	const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
 	chain_wait();
 	float s = 0.0f;
 	if (c < V)
 #pragma unroll 8
-		for (int k = y; k < row_blocks; k += 8) s += __ldg(col_part + (long long)k * ld + c);
+		for (int k = y; k < row_blocks; k += 8) s += col_part[(long long)k * ld + c];
 	tile[y][lane] = s;
 	__syncthreads();
 	if (y != 0 || c >= V) return;
@@ -190,8 +190,8 @@ __global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ 
 }
 
 // loss = sum of the row losses over their count, norm = 1 / count, in a fixed order in fp64.
-__global__ void __launch_bounds__(1024) ce_mean_kernel(long long rows, const float* __restrict__ row_loss,
-		const int* __restrict__ valid, float* __restrict__ loss, float* __restrict__ norm) {
+__global__ void __launch_bounds__(1024) ce_mean_kernel(long long rows, const float* row_loss,
+		const int* valid, float* loss, float* norm) {
 	__shared__ double sums[32];
 	__shared__ long long counts[32];
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

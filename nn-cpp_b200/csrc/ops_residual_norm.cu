@@ -157,7 +157,7 @@ struct Outs {
 
 // out (+)= the sum over a group's chunks: 32 columns per CTA, warp y of its eight sums chunks y, y + 8, ...
 // and the eight sums are added in order. grid = (ceil(D / 32), groups, arrays).
-__global__ void __launch_bounds__(256) residual_norm_params_kernel(const float* __restrict__ part, int chunks, int D,
+__global__ void __launch_bounds__(256) residual_norm_params_kernel(const float* part, int chunks, int D,
 		const Outs o) {
 	__shared__ float tile[8][32];
 	const int array = blockIdx.z, lane = threadIdx.x & 31, y = threadIdx.x >> 5;
@@ -172,12 +172,12 @@ __global__ void __launch_bounds__(256) residual_norm_params_kernel(const float* 
 		for (; c + 8 * 15 < chunks; c += 8 * 16) {       // sixteen loads in flight, added in order
 			float v[16];
 #pragma unroll
-			for (int k = 0; k < 16; ++k) v[k] = __ldg(src + (long long)(c + 8 * k) * D);
+			for (int k = 0; k < 16; ++k) v[k] = src[(long long)(c + 8 * k) * D];
 #pragma unroll
 			for (int k = 0; k < 16; ++k) s += v[k];
 		}
 #pragma unroll 4
-		for (; c < chunks; c += 8) s += __ldg(src + (long long)c * D);
+		for (; c < chunks; c += 8) s += src[(long long)c * D];
 	}
 	tile[y][lane] = s;
 	__syncthreads();
@@ -189,15 +189,15 @@ __global__ void __launch_bounds__(256) residual_norm_params_kernel(const float* 
 }
 
 // dgate row = its span's pieces in order. grid-stride over spans x D.
-__global__ void residual_norm_gate_kernel(const float* __restrict__ part, long long spans, int pieces, int D,
-		float* __restrict__ dgate, int first) {
+__global__ void residual_norm_gate_kernel(const float* part, long long spans, int pieces, int D,
+		float* dgate, int first) {
 	const long long total = spans * D;
 	chain_wait();
 	for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
 		const long long s = i / D;
 		const float* src = part + s * pieces * D + (i - s * D);
 		float v = 0.0f;
-		for (int k = 0; k < pieces; ++k) v += __ldg(src + (long long)k * D);
+		for (int k = 0; k < pieces; ++k) v += src[(long long)k * D];
 		dgate[i] = first ? v + 0.0f : dgate[i] + v;
 	}
 }

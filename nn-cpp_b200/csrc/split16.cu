@@ -39,7 +39,7 @@ struct RangeJobs {
 // grid.y: the groups of x, then w.
 __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 	const bool is_w = (int)blockIdx.y == jobs.groups;
-	const float* __restrict__ x = is_w ? jobs.w : jobs.x + blockIdx.y * jobs.n;
+	const float* x = is_w ? jobs.w : jobs.x + blockIdx.y * jobs.n;
 	const long long n = is_w ? jobs.nw : jobs.n;
 	const int vec = is_w ? jobs.vec_w : jobs.vec;
 	Range* out = jobs.out + blockIdx.y;
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 		const float4* x4 = reinterpret_cast<const float4*>(x);
 #pragma unroll 4
 		for (; i < n / 4; i += step) {
-			const float4 v = __ldg(x4 + i);
+			const float4 v = x4[i];
 			see(v.x);
 			see(v.y);
 			see(v.z);
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 		}
 	} else {
 #pragma unroll 4
-		for (; i < n; i += step) see(__ldg(x + i));
+		for (; i < n; i += step) see(x[i]);
 	}
 	top = __reduce_max_sync(0xffffffffu, top);
 	bad = __reduce_or_sync(0xffffffffu, bad);
@@ -95,9 +95,9 @@ struct PackJobs {
 // Four columns per thread: a float4 in (or four floats), 8 bytes of hi and of lo out. grid.y: the matrix.
 __global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
 	const PackWork& w = jobs.job[blockIdx.y];
-	const float* __restrict__ x = w.x;
-	unsigned char* __restrict__ out = w.out;
-	int* __restrict__ row_bad = w.row_bad;
+	const float* x = w.x;
+	unsigned char* out = w.out;
+	int* row_bad = w.row_bad;
 	const long long rows = w.rows, cols = w.cols, total = w.total;
 	const int vec = w.vec, parts = jobs.parts;
 	chain_wait();
@@ -117,12 +117,12 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
 		if (r < rows && c < cols) {
 			const float* src = x + r * cols + c;
 			if (vec) {
-				const float4 t = __ldg(reinterpret_cast<const float4*>(src));
+				const float4 t = *reinterpret_cast<const float4*>(src);
 				v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
 			} else {
 #pragma unroll
 				for (int k = 0; k < 4; ++k)
-					if (c + k < cols) v[k] = __ldg(src + k);
+					if (c + k < cols) v[k] = src[k];
 			}
 		}
 		bool bad = false;
@@ -426,10 +426,10 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 				// load, then broadcasts)
 				if (p.bias) {
 					float4 b;
-					b.x = n0 + 4 * lane < p.N ? __ldg(p.bias + n0 + 4 * lane) : 0.0f;
-					b.y = n0 + 4 * lane + 1 < p.N ? __ldg(p.bias + n0 + 4 * lane + 1) : 0.0f;
-					b.z = n0 + 4 * lane + 2 < p.N ? __ldg(p.bias + n0 + 4 * lane + 2) : 0.0f;
-					b.w = n0 + 4 * lane + 3 < p.N ? __ldg(p.bias + n0 + 4 * lane + 3) : 0.0f;
+					b.x = n0 + 4 * lane < p.N ? p.bias[n0 + 4 * lane] : 0.0f;
+					b.y = n0 + 4 * lane + 1 < p.N ? p.bias[n0 + 4 * lane + 1] : 0.0f;
+					b.z = n0 + 4 * lane + 2 < p.N ? p.bias[n0 + 4 * lane + 2] : 0.0f;
+					b.w = n0 + 4 * lane + 3 < p.N ? p.bias[n0 + 4 * lane + 3] : 0.0f;
 					st4[lane] = b;
 					__syncwarp();
 #pragma unroll
@@ -509,17 +509,17 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 }
 
 // c (+)= sum over slabs, in order; four floats per thread where aligned.
-__global__ void __launch_bounds__(256) sum_slabs_kernel(const float* __restrict__ slabs, int splits, long long n,
-		float* __restrict__ c, int accumulate, int vec) {
+__global__ void __launch_bounds__(256) sum_slabs_kernel(const float* slabs, int splits, long long n,
+		float* c, int accumulate, int vec) {
 	chain_wait();
 	const long long step = gridDim.x * 256LL;
 	long long i = blockIdx.x * 256LL + threadIdx.x;
 	if (vec) {
 		for (; i < n / 4; i += step) {
-			float4 a = __ldg(reinterpret_cast<const float4*>(slabs) + i);
+			float4 a = reinterpret_cast<const float4*>(slabs)[i];
 #pragma unroll 4
 			for (int k = 1; k < splits; ++k) {
-				const float4 b = __ldg(reinterpret_cast<const float4*>(slabs + k * n) + i);
+				const float4 b = reinterpret_cast<const float4*>(slabs + k * n)[i];
 				a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 			}
 			float4* d = reinterpret_cast<float4*>(c) + i;
@@ -531,8 +531,8 @@ __global__ void __launch_bounds__(256) sum_slabs_kernel(const float* __restrict_
 		}
 	} else {
 		for (; i < n; i += step) {
-			float a = __ldg(slabs + i);
-			for (int k = 1; k < splits; ++k) a += __ldg(slabs + k * n + i);
+			float a = slabs[i];
+			for (int k = 1; k < splits; ++k) a += slabs[k * n + i];
 			c[i] = accumulate ? c[i] + a : a;
 		}
 	}
