@@ -151,6 +151,10 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 	constexpr bool kBranch = kPost || kGate;       // the branch is read
 	constexpr int kStaged = staged_arrays(kBranch, VEC * KV);
 	constexpr int kStep = T * VEC;                 // floats between a thread's groups of VEC columns
+	// No load passes the wait for the staged row or a store. Single floats, and rows of 1024 threads, which have
+	// an SM to themselves, ask for gamma and the gate before those (16384 x 1001 87 -> 80 us, 2048 x 8192 103 -> 101);
+	// other rows leave that to the SM's other CTAs (32768 x 512 with post and gate 96 -> 87 without).
+	constexpr bool kAhead = VEC == 1 || T >= 1024;
 	const int slot = threadIdx.x / T, j0 = threadIdx.x % T * VEC;
 	const int D = p.D;
 	const float inv_d = 1.0f / (float)D;
@@ -205,6 +209,15 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 		const long long off = r * D + j0;
 		const float4 st = p.stats[r];
 		Pack<VEC> dt[KV], hat[KV], br[kBranch ? KV : 1];
+		Pack<VEC> gm[KV];
+		auto load_gamma = [&](int u) {
+			gm[u].zero();
+			if (in[u] && with_dy) gm[u].load(p.gamma + j0 + u * kStep);
+		};
+		if constexpr (kAhead) {
+#pragma unroll
+			for (int u = 0; u < KV; ++u) load_gamma(u);
+		}
 		float2 ab = make_float2(0.0f, 0.0f);
 		cp_async_wait<0>();
 #pragma unroll
@@ -223,18 +236,17 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 		if (with_dy) {
 #pragma unroll
 			for (int u = 0; u < KV; ++u) {
-				Pack<VEC> dy, g;
+				Pack<VEC> dy;
 				dy.zero();
-				g.zero();
 				hat[u].zero();
+				if constexpr (!kAhead) load_gamma(u);
 				if (in[u]) {
 					dy.load(stage + D + u * kStep);
 					hat[u].load(stage + 2 * D + u * kStep);
-					g.load(p.gamma + j0 + u * kStep);
 				}
 #pragma unroll
 				for (int i = 0; i < VEC; ++i) {
-					const float x = (hat[u].v[i] - st.x) * st.y, d = dy.v[i] * g.v[i];
+					const float x = (hat[u].v[i] - st.x) * st.y, d = dy.v[i] * gm[u].v[i];
 					hat[u].v[i] = x;
 					ab.x += d;
 					ab.y = __fmaf_rn(d, x, ab.y);
@@ -259,6 +271,15 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 #pragma unroll
 				for (int i = 0; i < VEC; ++i) dt[u].v[i] = dt[u].v[i] - ma - hat[u].v[i] * mb;
 		}
+		Pack<VEC> gt[kGate ? KV : 1];
+		auto load_gate = [&](int u) {
+			gt[u].zero();
+			if (in[u]) gt[u].load(gate_row + u * kStep);
+		};
+		if constexpr (kGate && kAhead) {
+#pragma unroll
+			for (int u = 0; u < KV; ++u) load_gate(u);
+		}
 		if (p.dx) {
 #pragma unroll
 			for (int u = 0; u < KV; ++u)
@@ -277,15 +298,13 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 				}
 			}
 			if constexpr (kGate) {
-				Pack<VEC> gt;
-				gt.zero();
-				if (in[u]) gt.load(gate_row + u * kStep);
+				if constexpr (!kAhead) load_gate(u);
 #pragma unroll
 				for (int i = 0; i < VEC; ++i) {
 					const float s = p.scale * dt[u].v[i];
 					const float pv = kPost ? __fmaf_rn((br[u].v[i] - st.z) * st.w, pg.v[i], pb.v[i]) : br[u].v[i];
 					sgate[u].v[i] = __fmaf_rn(s, pv, sgate[u].v[i]);
-					dt[u].v[i] = s * gt.v[i];
+					dt[u].v[i] = s * gt[u].v[i];
 				}
 			} else {
 #pragma unroll

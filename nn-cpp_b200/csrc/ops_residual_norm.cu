@@ -89,10 +89,17 @@ __device__ __forceinline__ void affine(Pack<VEC> (&a)[KV], const bool (&in)[KV],
 		for (int i = 0; i < VEC; ++i) a[u].v[i] = in[u] ? __fmaf_rn((a[u].v[i] - st.x) * st.y, g[u].v[i], b[u].v[i]) : 0.0f;
 }
 
+// CTAs per SM that the forward's registers must allow. Short rows live on occupancy: 32 registers where a thread
+// holds four columns (262144 x 64 53 us, 61 with 37 registers); two CTAs of 512 threads (2048 x 8192 49 us, 64 with
+// one); 80 registers for 16 columns (8190 x 2048 with post and gate 43 us, 49 with 99).
+__host__ __device__ constexpr int fwd_ctas(int cols, int t) {
+	return t == 1024 ? 1 : t == 512 ? 2 : cols <= 4 ? 8 : cols <= 8 ? 5 : 3;
+}
+
 // One row per slot of T threads, T and the columns per thread known to the compiler: the row's addresses
 // are one base and constant offsets, and the sums are straight code.
 template <int VEC, int KV, int T>
-__global__ void __launch_bounds__(T > kCta ? T : kCta) residual_norm_fwd_kernel(const Row p) {
+__global__ void __launch_bounds__(T > kCta ? T : kCta, fwd_ctas(VEC * KV, T)) residual_norm_fwd_kernel(const Row p) {
 	constexpr int kSlots = (T > kCta ? T : kCta) / T;
 	__shared__ float2 buf[2 * 32];
 	const int slot = threadIdx.x / T, t = threadIdx.x % T;
