@@ -17,7 +17,7 @@
 //
 // Both directions read every row once and keep it in registers: 16 bytes per element forward, 20 to 24
 // backward, so HBM bounds them (32768 x 512 layer: 39 us and 52 us, 6.9 and 6.5 TB/s; 8190 x 2048 rms with post
-// and gate: 43 and 75). T threads share a row (a power of two of warps, so that a thread holds
+// and gate: 43 and 73). T threads share a row (a power of two of warps, so that a thread holds
 // few columns); rows whose length is a multiple of 4 and whose buffers are 16-byte aligned move as
 // float4. In the backward each T-thread slot walks a run of consecutive rows and keeps its columns'
 // parameter sums in registers; the CTA's slots are summed in shared memory, and a second kernel sums
