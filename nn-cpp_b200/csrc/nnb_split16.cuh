@@ -51,6 +51,17 @@ inline size_t pack_bytes(long long rows, long long cols) {
 struct Range {
 	unsigned top, bad;
 };
+// The rows that count: those whose target is a token of the vocabulary and not `ignore` (targets null: all rows).
+// What the others hold takes no part in a range and is packed as zeros, so that it touches nothing.
+struct LiveRows {
+	const int64_t* targets = nullptr;
+	int64_t ignore = 0, V = 0;
+	__device__ __forceinline__ bool operator()(long long r) const {
+		if (!targets) return true;
+		const int64_t t = targets[r];
+		return t != ignore && t >= 0 && t < V;
+	}
+};
 // 2^k, -126 <= k <= 127.
 __device__ __forceinline__ float exp2_int(int k) { return __int_as_float((k + 127) << 23); }
 // s = 2^shift(range): the scale that puts the largest magnitude into [2^14, 2^15).
@@ -90,18 +101,21 @@ struct Product {
 	int* err = nullptr;
 };
 
-// Ranges of the `groups` runs of n values of x into out[0 .. groups), and of w[nw] into out[groups]; the caller
-// has zeroed them.
-nnb_status find_ranges(cudaStream_t s, const float* x, long long n, long long groups, const float* w, long long nw, Range* out);
+// Ranges of the `groups` runs of rows x cols values of x (the rows that `live` names) into out[0 .. groups), and
+// of w[nw] into out[groups]; the caller has zeroed them.
+nnb_status find_ranges(cudaStream_t s, const float* x, long long rows, long long cols, long long groups, LiveRows live,
+		const float* w, long long nw, Range* out);
 
 // A matrix to pack: x [rows x cols] (row-major, dense) into buf, rows padded with zeros to `row_blocks` blocks;
-// values that are not finite become zero and set row_bad[row] (nullable, zeroed by the caller).
+// rows that do not count become zeros, and values of others that are not finite become zero and set row_bad[row]
+// (nullable, zeroed by the caller).
 struct PackJob {
 	const float* x;
 	long long rows, cols, row_blocks;
 	const Range* range;
 	void* buf;
 	int* row_bad;
+	LiveRows live;
 };
 // One or two of them in one launch.
 nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts);

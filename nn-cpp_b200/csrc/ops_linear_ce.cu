@@ -329,7 +329,8 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 	int* valid = m.at<int>(l.valid);
 	const long long rg = c.P / c.groups;             // parameter gradients are kept per group of rows
 	NNB_CUDA_TRY(cudaMemsetAsync(ranges, 0, (size_t)(c.groups + 1) * sizeof(split16::Range) + (size_t)c.P * sizeof(int), s));
-	NNB_TRY(split16::find_ranges(s, c.x, rg * c.D, c.groups, c.w, c.V * c.D, ranges));
+	const split16::LiveRows live{c.targets, c.ignore_index, c.V};
+	NNB_TRY(split16::find_ranges(s, c.x, rg, c.D, c.groups, live, c.w, c.V * c.D, ranges));
 	split16::Pack W, X, G;
 	W.buf = m.at<void>(l.wpack); W.rows = c.V; W.cols = c.D;
 	for (long long z = 0; z < c.groups; ++z) {
@@ -339,8 +340,9 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 			const split16::Range* xr = ranges + z;
 			const float* x = c.x + r0 * c.D;
 			int* x_bad = m.at<int>(l.x_bad) + r0;
-			const split16::PackJob jobs[2] = {{x, n, c.D, blocks, xr, m.at<void>(l.xpack), x_bad},
-				{c.w, c.V, c.D, (c.V + 2 * kRows - 1) / (2 * kRows) * 2, wr, m.at<void>(l.wpack), nullptr}};
+			const split16::PackJob jobs[2] = {
+				{x, n, c.D, blocks, xr, m.at<void>(l.xpack), x_bad, {c.targets + r0, c.ignore_index, c.V}},
+				{c.w, c.V, c.D, (c.V + 2 * kRows - 1) / (2 * kRows) * 2, wr, m.at<void>(l.wpack), nullptr, {}}};
 			NNB_TRY(split16::pack(s, jobs, r0 == 0 ? 2 : 1, parts));           // W with the first piece
 			X.buf = m.at<void>(l.xpack); X.rows = n; X.cols = c.D;
 

@@ -31,17 +31,19 @@ namespace {
 
 struct RangeJobs {
 	const float *x, *w;
-	long long n, nw;                           // of each group of x, and of w
+	long long rows, cols, n, nw;               // of each group of x (n = rows cols), and of w
 	int vec, vec_w, groups;
+	LiveRows live;
 	Range* out;
 };
 
-// grid.y: the groups of x, then w.
+// grid.y: the groups of x, then w. A value of x counts if its row does.
 __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 	const bool is_w = (int)blockIdx.y == jobs.groups;
 	const float* x = is_w ? jobs.w : jobs.x + blockIdx.y * jobs.n;
-	const long long n = is_w ? jobs.nw : jobs.n;
+	const long long n = is_w ? jobs.nw : jobs.n, cols = jobs.cols, row0 = blockIdx.y * jobs.rows;
 	const int vec = is_w ? jobs.vec_w : jobs.vec;
+	const bool all = is_w || !jobs.live.targets;
 	Range* out = jobs.out + blockIdx.y;
 	chain_wait();
 	unsigned top = 0, bad = 0;
@@ -50,6 +52,7 @@ __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 		if (b >= 0x7f800000u) bad = 1;
 		else top = max(top, b);
 	};
+	auto row_of = [&](long long e) { return n < 0x7fffffffLL ? (long long)((unsigned)e / (unsigned)cols) : e / cols; };
 	const long long step = (long long)gridDim.x * blockDim.x;
 	long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
 	if (vec) {
@@ -57,6 +60,17 @@ __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 #pragma unroll 4
 		for (; i < n / 4; i += step) {
 			const float4 v = x4[i];
+			if (!all) {
+				const long long r = row_of(4 * i);
+				if (4 * i + 3 - r * cols >= cols) {          // these four lie in several rows
+					const float q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+					for (int k = 0; k < 4; ++k)
+						if (jobs.live(row0 + row_of(4 * i + k))) see(q[k]);
+					continue;
+				}
+				if (!jobs.live(row0 + r)) continue;
+			}
 			see(v.x);
 			see(v.y);
 			see(v.z);
@@ -64,7 +78,10 @@ __global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
 		}
 	} else {
 #pragma unroll 4
-		for (; i < n; i += step) see(x[i]);
+		for (; i < n; i += step) {
+			const float v = x[i];
+			if (all || jobs.live(row0 + row_of(i))) see(v);
+		}
 	}
 	top = __reduce_max_sync(0xffffffffu, top);
 	bad = __reduce_or_sync(0xffffffffu, bad);
@@ -86,6 +103,7 @@ struct PackWork {
 	const Range* range;
 	unsigned char* out;
 	int* row_bad;
+	LiveRows live;
 };
 struct PackJobs {
 	PackWork job[2];
@@ -114,7 +132,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
 		}
 		const long long c = q * 4;
 		float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-		if (r < rows && c < cols) {
+		if (r < rows && c < cols && w.live(r)) {
 			const float* src = x + r * cols + c;
 			if (vec) {
 				const float4 t = *reinterpret_cast<const float4*>(src);
@@ -583,9 +601,12 @@ nnb_status dispatch(cudaStream_t s, const DeviceState* dev, int epilogue, bool m
 
 }  // namespace
 
-nnb_status find_ranges(cudaStream_t s, const float* x, long long n, long long groups, const float* w, long long nw, Range* out) {
+nnb_status find_ranges(cudaStream_t s, const float* x, long long rows, long long cols, long long groups, LiveRows live,
+		const float* w, long long nw, Range* out) {
+	const long long n = rows * cols;
 	RangeJobs jobs;
-	jobs.x = x; jobs.n = n; jobs.groups = (int)groups; jobs.w = w; jobs.nw = nw; jobs.out = out;
+	jobs.x = x; jobs.rows = rows; jobs.cols = cols; jobs.n = n; jobs.groups = (int)groups; jobs.live = live;
+	jobs.w = w; jobs.nw = nw; jobs.out = out;
 	jobs.vec = n % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 	jobs.vec_w = nw % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 	const long long most = std::max(n, nw);
@@ -605,7 +626,7 @@ nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts) {
 		const PackJob& j = jobs[i];
 		PackWork& w = k.job[i];
 		w.x = j.x; w.rows = j.rows; w.cols = j.cols; w.range = j.range;
-		w.out = static_cast<unsigned char*>(j.buf); w.row_bad = j.row_bad;
+		w.out = static_cast<unsigned char*>(j.buf); w.row_bad = j.row_bad; w.live = j.live;
 		w.total = j.row_blocks * kRows * ((j.cols + kCols - 1) / kCols) * (kCols / 4);
 		w.vec = j.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(j.x) & 15) == 0;
 		most = std::max(most, w.total);

@@ -286,6 +286,46 @@ def test_ignored_rows_may_hold_anything(cuda):
     assert torch.equal(got[0], want[0]) and all(torch.equal(got[1][k], want[1][k]) for k in want[1])
 
 
+@pytest.mark.parametrize("P,D,V", [(40, 32, 64), (64, 33, 50), (7, 2, 20), (300, 1, 9), (2, 3, 5)])
+@pytest.mark.parametrize("value", [1e6, 1e20, 3e38])
+def test_rows_that_do_not_count_may_hold_large_values(cuda, P, D, V, value):
+    """What a row with an ignored target holds leaves every bit of the loss and the gradients alone, with rows
+    that share a 16-byte load among them; so does a row whose target is no token, for the gradients."""
+    x, w, b, t = _make(P, D, V, seed=21)
+    dead = [i for i in range(P) if i % 3 == 1]
+    t[dead] = IGNORE
+    want = _run(x, w, b, t)
+    _close(want[0], _want(x, w, b, t, 0.0)["loss"], "loss")
+    x2 = x.clone()
+    x2[dead] = value
+    got = _run(x2, w, b, t)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(got[1][k], want[1][k]) for k in want[1])
+    rows = [F.linear_token_losses(*[Value.leaf(v, False) for v in (data, w, b)], t)[0] for data in (x, x2)]
+    assert torch.equal(*rows)
+    t2 = t.clone()
+    t2[dead] = V
+    loss, grads = _run(x2, w, b, t2)
+    assert torch.isnan(loss).all() and nnb.device_error() == 16
+    assert all(torch.equal(grads[k], want[1][k]) for k in want[1])
+
+
+def test_ignored_rows_of_a_group_may_hold_large_values(cuda):
+    G, P, D, V = 2, 2 * 36, 5, 30
+    x, w, b, t = _make(P, D, V, seed=22)
+    t[[3, 50]] = IGNORE
+    norm = torch.tensor([1.0 / 36], device="cuda")
+    out = []
+    for value in (1.0, 1e30):
+        x[[3, 50]] = value
+        vals = {"x": Value.leaf(x, True), "w": Value.leaf(w, True), "b": Value.leaf(b, True)}
+        for k, n in (("w", V * D), ("b", V)):
+            vals[k].grad, vals[k].grad_fresh = torch.empty(G, n, device="cuda"), True
+        with F.param_groups(G):
+            F.linear_cross_entropy(vals["x"], vals["w"], vals["b"], t, grad_norm=norm).backward()
+        out.append([v.grad for v in vals.values()])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
 def test_tf32_mode(cuda):
     """The fast mode: operands of 11 significant bits, 2^-11 of each term's two factors."""
     x, w, b, t = _make(300, 64, 500, seed=11)
