@@ -43,11 +43,38 @@ def param_groups(n: int):
         _GROUPS = old
 
 
+def _holds_groups(buf, n: int) -> bool:
+    """Whether a gradient buffer has room for the current groups' gradients of n elements each."""
+    if _GROUPS == 1:
+        return buf.numel() == n
+    if buf.numel() != _GROUPS * n:
+        return False
+    return buf.is_contiguous() or (buf.dim() == 2 and buf.shape[0] == _GROUPS and buf.stride(0) >= n and
+                                   (n == 1 or buf.stride(1) == 1))
+
+
 def _gstride(buf, param: Value) -> int:
     """Elements between consecutive groups' gradients in a parameter's gradient buffer."""
     if buf is None:
         return 0
-    return buf.stride(0) if buf.dim() == 2 and buf.shape[0] == _GROUPS and _GROUPS > 1 else param.data.numel()
+    n = param.data.numel()
+    if _GROUPS == 1:
+        return n
+    if not _holds_groups(buf, n):
+        raise TensorShapeError(f"a gradient buffer of shape {tuple(buf.shape)} cannot hold {_GROUPS} groups of {n} elements")
+    return buf.stride(0) if buf.dim() == 2 and buf.shape[0] == _GROUPS else n
+
+
+def _check_grouped(who: str, params) -> None:
+    """Refuses a backward rule whose parameters' gradient buffers are not laid out for the current parameter
+    groups, before any of them is taken (grad_accum would mark it as written)."""
+    for p in params:
+        if p is None or not p.requires_grad:
+            continue
+        buf = p.data if p.grad is None or p.grad_borrowed else p.grad       # (grad_accum makes one like the data)
+        if (_GROUPS > 1 or buf.shape != p.data.shape) and not _holds_groups(buf, p.data.numel()):
+            raise TensorShapeError(f"{who}: a gradient buffer of shape {tuple(buf.shape)} does not hold {_GROUPS} group(s) of "
+                                   f"{p.data.numel()} elements")
 
 
 # ---- linear (ops.cpp:714-745) -------------------------------------------------------------------
@@ -407,6 +434,8 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     held = []          # (backward pass, what reached y in it)
 
     def run(dh, dy):
+        _check_grouped("residual_norm", (gamma, beta, post_gamma, post_beta, gate if gate_rows == 1 else None))
+
         def out(v, grouped):
             if v is None or not _need(v):
                 return None
@@ -451,6 +480,7 @@ def rmsnorm(x: Value, gamma: Value, eps: float) -> Value:
                                       None, None, _p(y), _p(stats)))
 
     def backward(g):
+        _check_grouped("rmsnorm", (gamma,))
         dx, fx = x.grad_accum() if _need(x) else (None, 0)
         dg, fg = gamma.grad_accum() if _need(gamma) else (None, 0)
         check(lib().nnb_residual_norm_bwd(_s(), R, D, _GROUPS, 0, NORM_RMS, 1.0, None, _p(g), _p(x.data), None, None, None,
@@ -893,12 +923,20 @@ def linear_cross_entropy(x: Value, weight: Value, bias: Value | None, targets: t
                                   0, at[2], 0))
 
     def backward(g):
+        if params and groups != _GROUPS:
+            raise ValueError(f"linear_cross_entropy: the forward kept gradients for {groups} parameter group(s), the "
+                             f"backward runs in {_GROUPS}")
+        if params:
+            _check_grouped("linear_cross_entropy", parents[1:])
+        runs = (1, groups, groups)
+        if any(n and n != v.data.numel() * k for v, n, k in zip((x, weight, bias), sizes, runs)):
+            raise TensorShapeError("linear_cross_entropy: an operand changed its size since the forward")
         grads = []
-        for v, n, lo in zip((x, weight, bias), sizes, starts):
+        for v, n, lo, runs_of in zip((x, weight, bias), sizes, starts, runs):
             if n:
                 buf, f = v.grad_accum()
-                own = v.data.numel()
-                grads.append(ScaledGrad(kept.data_ptr() + 4 * lo, buf.data_ptr(), own, n // own, _gstride(buf, v), f))
+                grads.append(ScaledGrad(kept.data_ptr() + 4 * lo, buf.data_ptr(), n // runs_of, runs_of,
+                                        _gstride(buf, v) if runs_of > 1 else 0, f))
         k = norm_at if grad_norm is None else grad_norm.data_ptr()
         # (one launch, unless x is the weight itself: then its two gradients are added one after the other)
         for part in ([grads] if x is not weight else [[e] for e in grads]):

@@ -65,3 +65,33 @@ def test_grad_norm_refusals():
     for bad in (torch.ones(2), torch.ones(0)):
         with pytest.raises(TensorShapeError, match="one value"):
             F.linear_cross_entropy(*args, grad_norm=bad)
+
+
+def test_gradient_buffers_and_groups():
+    """Buffers that the current parameter groups do not fit are refused without being marked as written."""
+    def leaf(shape, grad):
+        v = Value.leaf(torch.zeros(shape), True)
+        v.grad = torch.zeros(grad) if grad else None
+        return v
+
+    for groups, shape, grad, fits in ((1, (4, 8), (4, 8), True), (1, (4, 8), (1, 32), True), (1, (4, 8), None, True),
+                                      (1, (4, 8), (4, 32), False), (4, (4, 8), (4, 8), False), (4, (4, 8), None, False),
+                                      (4, (4, 8), (4, 32), True), (4, (4, 8), (4, 4, 8), True), (4, (4, 8), (3, 32), False),
+                                      (4, (1,), (4, 1), True)):
+        v = leaf(shape, grad)
+        with F.param_groups(groups):
+            if fits:
+                F._check_grouped("op", (None, v, Value(torch.zeros(3))))
+                assert F._gstride(v.grad, v) == (v.data.numel() if grad else 0)
+            else:
+                with pytest.raises(TensorShapeError, match="does not hold"):
+                    F._check_grouped("op", (v,))
+                if groups > 1 and grad:
+                    with pytest.raises(TensorShapeError, match="cannot hold"):
+                        F._gstride(v.grad, v)
+        assert v.grad_fresh
+    v = leaf((4, 8), (4, 32))
+    v.grad = torch.zeros(4, 40)[:, :32]                  # views of a flat buffer, as the sharded trainer's
+    with F.param_groups(4):
+        F._check_grouped("op", (v,))
+        assert F._gstride(v.grad, v) == 40

@@ -258,6 +258,42 @@ def test_parameter_groups(cuda):
         assert torch.equal(vals["w"].grad[z].view(V, D), part["w"]) and torch.equal(vals["b"].grad[z], part["b"])
 
 
+def test_backward_outside_the_forwards_groups(cuda):
+    """The kept gradients have the forward's groups: a backward in other groups, or into buffers that do not hold
+    them, is refused before anything is launched or marked as written."""
+    G, P, D, V = 2, 2 * 8, 6, 10
+    x, w, b, t = _make(P, D, V, seed=19)
+
+    def forward(grouped):
+        vals = [Value.leaf(v, True) for v in (x, w, b)]
+        if grouped:
+            for v in vals[1:]:
+                v.grad = torch.empty(G, v.data.numel(), device="cuda")
+        return vals, lambda: F.linear_cross_entropy(*vals, t)
+
+    def refused(vals, loss, match):
+        with pytest.raises(ValueError, match=match):
+            loss.backward()
+        assert all(v.grad_fresh for v in vals)
+
+    vals, f = forward(False)
+    with F.param_groups(G):
+        loss = f()
+    refused(vals, loss, "parameter group")
+    vals, f = forward(True)
+    loss = f()
+    with F.param_groups(G):
+        refused(vals, loss, "parameter group")
+    for inside in (True, False):       # buffers that do not fit the groups
+        vals, f = forward(not inside)
+        with F.param_groups(G if inside else 1):
+            refused(vals, f(), "does not hold")
+    vals, f = forward(True)
+    with F.param_groups(G):
+        f().backward()
+    assert torch.equal(vals[0].grad, _run(x, w, b, t)[1]["x"])
+
+
 def test_groups_of_different_size(cuda):
     """A group's bits are its own whatever the other groups hold: here one 2^30 times larger, next to values
     that its scale would have lost."""

@@ -253,6 +253,29 @@ def test_parameter_groups(cuda):
         assert torch.equal(vals["gate"].grad[spans], grads["gate"])
 
 
+def test_gradients_that_the_groups_do_not_fit(cuda):
+    """Parameters whose buffers do not hold the backward's groups, an activation used as one among them, are
+    refused before a gradient is taken."""
+    G, R, D = 2, 8, 12
+    ops, dh, dy = _make(R, D, R, "rms", False, "channel", seed=31)
+    for bad in ("gamma", "gate"):
+        vals = {k: Value.leaf(v, True) for k, v in ops.items()}
+        for k in ("gamma", "gate"):
+            if k != bad:
+                vals[k].grad = torch.empty(G, D, device="cuda")
+        if bad == "gate":
+            vals["gate"] = F.add(vals["gate"], vals["gate"])
+        with F.param_groups(G):
+            h, y = F.residual_norm(vals["x"], vals["branch"], vals["gamma"], None, EPS, kind="rms", gate=vals["gate"])
+            with pytest.raises(ValueError, match="does not hold"):
+                backward((h, y), (dh, dy))
+        assert vals["x"].grad_fresh and vals["branch"].grad_fresh and vals["gamma"].grad_fresh
+    x, gamma = Value.leaf(ops["x"], True), Value.leaf(ops["gamma"], True)
+    with F.param_groups(G), pytest.raises(ValueError, match="does not hold"):
+        F.rmsnorm(x, gamma, EPS).backward(dy)
+    assert x.grad_fresh and gamma.grad_fresh
+
+
 def test_gradients_against_differences(cuda):
     """Along a random direction: the 64-bit function's central difference and the operator's gradients.
     The difference's own error is step^2 / 6 of a third derivative, far below the 1e-4 allowed."""
