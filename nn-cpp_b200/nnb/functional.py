@@ -420,6 +420,9 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
             raise TensorShapeError("residual_norm: the gate's rows do not divide into the parameter groups")
     if R % _GROUPS:
         raise TensorShapeError("residual_norm: the rows do not divide into the parameter groups")
+    params = [v for v in (gamma, beta, post_gamma, post_beta, gate if gate_rows == 1 else None) if v is not None and _need(v)]
+    if len({id(v) for v in params}) != len(params):
+        raise ValueError("residual_norm: one parameter in two places, whose gradients would go to one buffer")
     _check_buffers("residual_norm", (x, branch, gamma, beta, post_gamma, post_beta, gate))
     k = NORM_LAYER if layer else NORM_RMS
     opt = lambda v: None if v is None else v.data.data_ptr()
@@ -434,7 +437,7 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     held = []          # (backward pass, what reached y in it)
 
     def run(dh, dy):
-        _check_grouped("residual_norm", (gamma, beta, post_gamma, post_beta, gate if gate_rows == 1 else None))
+        _check_grouped("residual_norm", params)
 
         def out(v, grouped):
             if v is None or not _need(v):

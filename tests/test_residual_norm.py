@@ -83,6 +83,20 @@ def test_function_refusals():
         F.residual_norm(x, b, g, be)
 
 
+def test_one_parameter_in_two_places():
+    """Refused when the sum is built, before any gradient buffer is taken; where no gradient is wanted the check of
+    the buffers is the next."""
+    x, b, be, be2 = _values((2, 3, 8), (2, 3, 8), (8,), (8,))
+    for train, match in ((True, "two places"), (False, "current CUDA device")):
+        g, row = Value.leaf(torch.ones(8), train), Value.leaf(torch.ones(1, 8), train)
+        with pytest.raises(ValueError, match=match):
+            F.residual_norm(x, b, g, be, post_gamma=g, post_beta=be2)
+        with pytest.raises(ValueError, match=match):
+            F.residual_norm(x, b, g, kind="rms", gate=g)
+        with pytest.raises(ValueError, match="current CUDA device"):
+            F.residual_norm(x, b, g, kind="rms", gate=row)
+
+
 def test_rmsnorm_refusals():
     x, g = _values((3, 8), (8,))
     for args in ((x, _values((7,))[0], 1e-5), (_values((0, 8))[0], g, 1e-5)):
