@@ -396,8 +396,9 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
     channel (its gradient kept per parameter group as a norm's is), [N, 1, D] one row per sequence of an
     x of [N, T, D], x's own shape one per token.
 
-    The backward runs when h's turn comes, with what reached y held until then: the gradient buffer of h
-    itself keeps what its other consumers gave."""
+    The backward runs when h's turn comes, with what reached y held until then. h's whole gradient is formed in
+    registers on the way to x's and the branch's: h.grad, whose buffer held only what h's other consumers gave, is
+    None after a backward pass."""
     if kind not in ("layer", "rms"):
         raise ValueError('residual_norm: kind must be "layer" or "rms"')
     layer = kind == "layer"
@@ -457,6 +458,8 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
             dy = None
         node = h_ref()
         run(None if node is not None and node.grad_fresh else g, dy)
+        if node is not None:
+            node.grad, node.grad_fresh, node.grad_borrowed = None, False, False
 
     def y_backward(g):
         if h.requires_grad:

@@ -253,6 +253,28 @@ def test_parameter_groups(cuda):
         assert torch.equal(vals["gate"].grad[spans], grads["gate"])
 
 
+@pytest.mark.parametrize("roots", ["y", "hy", "h", "consumer"])
+def test_no_partial_gradient_is_left_on_h(cuda, roots):
+    """h's whole gradient is never stored: h.grad is None after a pass, and passes over the same graph repeat."""
+    ops, dh, dy = _make(6, 20, 6, "layer", False, "none", seed=33)
+    vals = {k: Value.leaf(v, True) for k, v in ops.items()}
+    h, y = F.residual_norm(vals["x"], vals["branch"], vals["gamma"], vals["beta"], EPS)
+    other = F.add(h, y)
+    seen = []
+    for _ in range(2):
+        for v in vals.values():
+            v.zero_grad()
+        if roots == "consumer":
+            other.backward(dh)
+        else:
+            backward([{"h": h, "y": y}[r] for r in roots], [{"h": dh, "y": dy}[r] for r in roots])
+        assert h.grad is None
+        seen.append([v.grad.clone() for k, v in vals.items() if roots != "h" or k in ("x", "branch")])
+    assert all(torch.equal(a, b) for a, b in zip(*seen))
+    _check(ops, h.data, y.data, {k: v.grad for k, v in vals.items() if roots != "h" or k in ("x", "branch")},
+           dh if roots != "y" else None, dh if roots == "consumer" else dy if "y" in roots else None, "layer", 1.0)
+
+
 def test_gradients_that_the_groups_do_not_fit(cuda):
     """Parameters whose buffers do not hold the backward's groups, an activation used as one among them, are
     refused before a gradient is taken."""
