@@ -529,6 +529,12 @@ def _addresses(who: str, tensors, sizes) -> list[int]:
     return out
 
 
+def _apart(addresses, sizes) -> bool:
+    """Whether fp32 buffers of the given addresses and sizes share no memory."""
+    spans = sorted((a, a + 4 * n) for a, n in zip(addresses, sizes) if n)
+    return all(end <= start for (_, end), (start, _) in zip(spans, spans[1:]))
+
+
 def _pointers(addresses):
     return (ctypes.c_void_p * len(addresses))(*addresses)
 
@@ -574,6 +580,7 @@ class AdamW:
         self.m, self.v = (tuple(flat[o: o + n].view(p.data.shape) for p, n, o in zip(self.params, sizes, self.offsets))
                           for flat in (self.flat_m, self.flat_v))
         self._sizes, self._n = sizes, (ctypes.c_size_t * len(sizes))(*sizes)
+        self._at, self._at_apart = None, False       # parameter addresses of the last step, and whether they are apart
         self._states = [_pointers([t.data_ptr() for t in ts]) for ts in (self.m, self.v)]
         if state_bits == 8:
             self.unit_m, self.unit_v = (zeros(total // self.BLOCK, torch.float32) for _ in range(2))
@@ -667,10 +674,11 @@ class AdamW:
         update = lib().nnb_adamw_multi_step if self.state_bits == 32 else lib().nnb_adamw8_multi_step
         scalars = (self.lr, self.beta1, self.beta2, self.eps, self.weight_decay)
         self.t += 1
-        used = [a for a, n in zip(w, self._sizes) if n]
-        if len(set(used)) == len(used):
+        if w != self._at:
+            self._at, self._at_apart = w, _apart(w, self._sizes)
+        if self._at_apart:
             check(update(s, len(w), self._n, _pointers(w), _pointers(g), *self._states, *scalars, self.t))
             return
-        for i in range(len(w)):      # a parameter listed twice is updated twice, one after the other
+        for i in range(len(w)):      # a parameter listed twice, or that shares memory: one after the other, in order
             check(update(s, 1, (ctypes.c_size_t * 1)(self._n[i]), _pointers(w[i: i + 1]), _pointers(g[i: i + 1]),
                          *(_pointers(ps[i: i + 1]) for ps in self._states), *scalars, self.t))

@@ -56,3 +56,9 @@ def test_optimizer_refusals():
         nn.AdamW([], state_bits=16)
     with pytest.raises(ValueError, match="current CUDA device"):
         nn.AdamW([Value(torch.zeros(4))])
+
+
+def test_buffers_that_share_memory():
+    apart = nn._apart
+    assert apart([], []) and apart([64], [16]) and apart([128, 64], [4, 16]) and apart([64, 64, 96], [0, 8, 4])
+    assert not apart([64, 64], [4, 4]) and not apart([124, 64], [4, 16]) and not apart([64, 80, 400], [100, 1, 3])

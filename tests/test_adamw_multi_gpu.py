@@ -177,6 +177,27 @@ def test_null_gradient_is_zeros(cuda):
         assert torch.equal(oa.flat_m, ob.flat_m) and torch.equal(oa.flat_v, ob.flat_v)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_share_memory(cuda, bits):
+    """Slices of one buffer that overlap are updated one after the other in the list's order, each with its own
+    moments, as one step per entry does."""
+    runs = []
+    for together in (True, False):
+        g = torch.Generator(device="cuda").manual_seed(8)
+        flat = torch.randn(20000, generator=g, device="cuda")
+        params = []
+        for lo, hi in ((0, 9000), (300, 20000), (100, 101), (8999, 9100)):
+            params.append(Value(flat[lo:hi], True))
+            params[-1].grad = torch.randn(hi - lo, generator=g, device="cuda")
+        opts = [nn.AdamW(params, **HYPER, state_bits=bits)] if together else \
+            [nn.AdamW([p], **HYPER, state_bits=bits) for p in params]
+        for _ in range(3):
+            for opt in opts:
+                opt.step()
+        runs.append([flat] + [t for k in ("m", "v") for opt in opts for t in getattr(opt, k)])
+    assert len(runs[0]) == 9 and all(torch.equal(a, b) for a, b in zip(*runs))
+
+
 def test_same_parameter_twice(cuda):
     """A parameter listed twice is updated twice in order, as one step per entry does."""
     p, = _params([1000], 17)
