@@ -192,8 +192,7 @@ __device__ __forceinline__ void load_block(Block8& b, bool vec, int n, int lane,
 }
 
 // The step on a loaded block, its new units and its stores. The root r' = sqrt(v') serves both the
-// update, w - (lr / c1) m' / (r' / sqrt(c2) + eps), and the stored code. The update's division is the
-// approximate one (2 ulp of a step that is small next to w).
+// update, w - (lr / c1) m' / (r' / sqrt(c2) + eps), and the stored code.
 //
 // Units: as unsigned integers the bit patterns of magnitudes order as the values do, NaN above infinity,
 // so a block that holds a NaN or an infinity gets such a unit and reads back as not finite throughout.
@@ -209,9 +208,7 @@ __device__ __forceinline__ void step_block(Block8& b, const Scalars& s, bool vec
 		const float r0 = kr * kr * b.vu, g = b.g[q];
 		mv[q] = s.b1 * decode(km, b.mu) + s.keep1 * g;
 		rv[q] = sqrtf(s.b2 * (r0 * r0) + s.keep2 * g * g);
-		float rcp;
-		asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rcp) : "f"(__fmaf_rn(rv[q], s.inv_root_c2, s.eps)));
-		b.w[q] = __fmaf_rn(s.minus_lr_c1 * mv[q], rcp, b.w[q] * s.shrink);
+		b.w[q] = b.w[q] * s.shrink + s.minus_lr_c1 * mv[q] / __fmaf_rn(rv[q], s.inv_root_c2, s.eps);
 		top_m = max(top_m, __float_as_uint(mv[q]) & 0x7fffffffu);
 		top_r = max(top_r, __float_as_uint(rv[q]) & 0x7fffffffu);
 	}
@@ -260,10 +257,12 @@ __device__ __forceinline__ void step_block(Block8& b, const Scalars& s, bool vec
 }
 
 // One block per warp, in small CTAs: 56 registers leave 36 warps on an SM, whose loads cover HBM's
-// latency and each other's arithmetic (about 70 instructions per element, two thirds of what the issue
-// slots give in the time HBM needs). 2^27 elements: 370 us, 5.8 TB/s, 0.89 of the measured copy rate.
-// Measured against it: CTAs of 256 threads 384 to 394 us; several blocks per warp, even with the next
-// block's loads issued ahead, 400 to 850 us (the warps drift apart in a long loop body).
+// latency and each other's arithmetic (about 80 instructions per element, most of what the issue
+// slots give in the time HBM needs). 2^27 elements: 398 us, 5.4 TB/s, 0.82 of the measured copy rate; with an
+// approximate reciprocal in place of the update's division 371 us, but the update is held to the 32-bit
+// step's roundings. Measured against it: 64 registers and 32 warps 404 us; CTAs of 256 threads 4 to 6 %
+// slower; several blocks per warp, even with the next block's loads issued ahead, 8 to 130 % slower (the
+// warps drift apart in a long loop body).
 template <int kCap>
 __global__ void __launch_bounds__(kThreads8, 9) adamw8_multi_kernel(const __grid_constant__ List8<kCap> l) {
 	const int ti = find_tensor(l, blockIdx.x);

@@ -177,6 +177,24 @@ def test_null_gradient_is_zeros(cuda):
         assert torch.equal(oa.flat_m, ob.flat_m) and torch.equal(oa.flat_v, ob.flat_v)
 
 
+@pytest.mark.parametrize("n", [512, 256 * 5 + 77])
+def test_8bit_update_is_rounded_like_the_32bit_one(cuda, n):
+    """The first step from weights of zero and without eps is its quotient alone, every operation in it rounded to
+    nearest: numpy's fp32 arithmetic gives the same bits."""
+    f = np.float32
+    g = torch.randn(n, generator=torch.Generator(device="cuda").manual_seed(41), device="cuda")
+    p = Value(torch.zeros(n, device="cuda"), True)
+    p.grad = g
+    nn.AdamW([p], lr=3e-3, beta1=0.9, beta2=0.999, eps=0.0, weight_decay=0.0, state_bits=8).step()
+    b1, b2, gn = f(0.9), f(0.999), g.cpu().numpy()
+    c1, c2 = f(1) - b1, f(1) - b2
+    m = (f(1) - b1) * gn
+    r = np.sqrt((f(1) - b2) * gn * gn)
+    want = (-f(3e-3) / c1 * m) / (r * (f(1) / np.sqrt(c2)))
+    assert want.dtype == np.float32
+    assert np.array_equal(p.data.cpu().numpy().view(np.int32), want.view(np.int32))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_parameters_that_share_memory(cuda, bits):
     """Slices of one buffer that overlap are updated one after the other in the list's order, each with its own
