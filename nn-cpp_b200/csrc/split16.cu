@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 	constexpr int kStages = stages(kParts), kStageBytes = stage_bytes(kParts);
 	extern __shared__ uint8_t smem_raw[];
 	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-	__shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], accf_bar[2], acce_bar[2];
+	__shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], accf_bar[2], acce_bar[2], drain_bar;
 	__shared__ uint32_t tmem_base_sh;
 	__shared__ int abort_sh;
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 			mbar_init(smem_u32(&accf_bar[b]), 1);
 			mbar_init(smem_u32(&acce_bar[b]), kEpiWarps);
 		}
+		mbar_init(smem_u32(&drain_bar), 1);
 		abort_sh = 0;
 		fence_mbar_init();
 		tma_prefetch_desc(&tm_a);
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 			// ------------------------------ TMA producer ------------------------------
 			int stage = 0;
 			uint32_t phase = 0;
-			bool ok = true;
+			bool ok = true, wrapped = false;
 			for (int t = blockIdx.x; ok && t < items; t += gridDim.x) {
 				const Item it = item_at(t, p);
 				for (int kb = it.kb0; kb < it.kb1; ++kb) {
@@ -296,9 +297,15 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 					if (++stage == kStages) {
 						stage = 0;
 						phase ^= 1;
+						wrapped = true;
 					}
 				}
 			}
+			// every issued copy has landed before the CTA can exit, on the way out of a wait that gave up too: the
+			// last one into each stage, those before `stage` in this round through the stages and the rest in the last
+			for (int s = 0; s < kStages; ++s)
+				if (s < stage || wrapped)
+					mbar_wait(smem_u32(&full_bar[s]), s < stage ? phase : phase ^ 1, p.err, kDevTimeoutDrain, nullptr);
 		} else if (warp == 1) {
 			// --------------------- MMA issuer (the whole warp; one elected lane issues) ---------------------
 			constexpr uint32_t idesc = idesc_f16(kBM, kBN) | (kMnA ? kIdescAMajorMN : 0u) | (kMnB ? kIdescBMajorMN : 0u);
@@ -349,6 +356,9 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 					if (ok) mma_commit_elect(smem_u32(&accf_bar[v & 1]));
 				}
 			}
+			// and every issued MMA has finished before the stages and tensor memory are released
+			mma_commit_elect(smem_u32(&drain_bar));
+			mbar_wait_warp(smem_u32(&drain_bar), 0, p.err, kDevTimeoutDrain, nullptr);
 		}
 	} else {
 		asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
