@@ -15,6 +15,10 @@ namespace resnorm {
 constexpr int kCta = 256;                // threads of a CTA whose rows need at most that many
 constexpr int kMaxD = 16384;             // columns that 1024 threads hold, 16 each
 constexpr int kArrays = 5;               // parameter sums: gamma, beta, post gamma, post beta, gate
+// Sums of the forms are kept back to back: where the sum `array` of a form is, or how many there are (kArrays).
+__host__ __device__ constexpr int sum_index(int array, bool layer, bool post, bool gate_param) {
+	return (array > 0) + (array > 1 && layer) + (array > 2 && post) + (array > 3 && post && layer) + (array > 4 && gate_param);
+}
 // CTAs per SM that the backward's registers allow: rows of at most 256 threads three (80 registers), two
 // with a gate or post's norm (128: their sums and operands); longer rows one (128 or 64 registers)
 __host__ __device__ constexpr int bwd_ctas(bool sums, int max_t) { return max_t > kCta ? 1 : sums ? 2 : 3; }
@@ -31,7 +35,7 @@ struct Grad {
 	// one of `pieces` pieces of `run_rows` rows of one span
 	long long group_rows, span, run_rows, spans_per_run, pieces, runs;
 	int chunks;                          // CTAs per group
-	float* part;                         // [kArrays][groups][chunks][D]
+	float* part;                         // [the form's sums][groups][chunks][D]
 	float* gate_part;                    // [groups * runs][D], pieces of a span
 };
 
@@ -385,12 +389,13 @@ __global__ void __launch_bounds__(T > kCta ? T : kCta, bwd_ctas(kPost || kGate, 
 		}
 		__syncthreads();
 	};
-	flush(sg, 0);
-	if constexpr (kLayer) flush(sb, 1);
-	if constexpr (kPost) flush(spg, 2);
-	if constexpr (kPost && kLayer) flush(spb, 3);
+	constexpr auto at = [](int array) { return sum_index(array, kLayer, kPost, kGate); };
+	flush(sg, at(0));
+	if constexpr (kLayer) flush(sb, at(1));
+	if constexpr (kPost) flush(spg, at(2));
+	if constexpr (kPost && kLayer) flush(spb, at(3));
 	if constexpr (kGate) {
-		if (p.gate_is_param) flush(sgate, 4);
+		if (p.gate_is_param) flush(sgate, at(4));
 	}
 }
 

@@ -363,7 +363,8 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 	p.chunks = (int)chunks;
 
 	const bool gate_pieces = gate && !gate_param && p.pieces > 1;
-	const size_t part = (size_t)kArrays * groups * chunks * D, gpart = gate_pieces ? (size_t)groups * p.runs * D : 0;
+	const size_t part = (size_t)sum_index(kArrays, p.layer, post_gamma != nullptr, gate_param) * groups * chunks * D;
+	const size_t gpart = gate_pieces ? (size_t)groups * p.runs * D : 0;
 	void* ws = nullptr;
 	NNB_TRY(scratch_alloc(&ws, (part + 3 + gpart) * sizeof(float), s));
 	p.part = static_cast<float*>(ws);
@@ -377,13 +378,14 @@ nnb_status nnb_residual_norm_bwd(void* stream, size_t R, size_t D, size_t groups
 	Outs o;
 	bool any = false;
 	int arrays = 0;
+	const bool kept[kArrays] = {true, p.layer != 0, post_gamma != nullptr, post_gamma && p.layer, gate_param};
 	for (int i = 0; i < kArrays; ++i) {
-		const bool computed = i < 2 || (i < 4 ? post_gamma != nullptr : gate_param);
-		o.out[i] = computed ? outs[i].p : nullptr;
-		o.stride[i] = (long long)(outs[i].stride ? outs[i].stride : D);
-		o.first[i] = outs[i].first;
-		if (o.out[i]) arrays = i + 1;
-		any |= o.out[i] != nullptr;
+		if (!kept[i]) continue;
+		o.out[arrays] = outs[i].p;
+		o.stride[arrays] = (long long)(outs[i].stride ? outs[i].stride : D);
+		o.first[arrays] = outs[i].first;
+		any |= outs[i].p != nullptr;
+		++arrays;
 	}
 	if (st == NNB_OK && any) {
 		TraceScope ts(s, kTraceRowwise);
