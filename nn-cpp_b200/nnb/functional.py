@@ -423,7 +423,7 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
         raise TensorShapeError("residual_norm: the rows do not divide into the parameter groups")
     params = [v for v in (gamma, beta, post_gamma, post_beta, gate if gate_rows == 1 else None) if v is not None and _need(v)]
     if len({id(v) for v in params}) != len(params):
-        raise ValueError("residual_norm: one parameter in two places, whose gradients would go to one buffer")
+        raise ValueError("residual_norm: one parameter in two places would share a gradient buffer")
     _check_buffers("residual_norm", (x, branch, gamma, beta, post_gamma, post_beta, gate))
     k = NORM_LAYER if layer else NORM_RMS
     opt = lambda v: None if v is None else v.data.data_ptr()
