@@ -322,6 +322,27 @@ def test_ignored_rows_may_hold_anything(cuda):
     assert torch.equal(got[0], want[0]) and all(torch.equal(got[1][k], want[1][k]) for k in want[1])
 
 
+@pytest.mark.parametrize("std", [30.0, 300.0])
+def test_gradients_of_large_logits(cuda, std):
+    """Gradients of a softmax that is close to one-hot, and one-hot, against their bounds."""
+    x, w, b, t = _make(16, 64, 200, seed=9)
+    _, grads = _run(x * std, w * std, b, t)
+    want = _want(x * std, w * std, b, t, 0.0)
+    for k, got in grads.items():
+        _close(got, want[k], k)
+
+
+def test_gradients_of_confident_rows(cuda):
+    """Rows whose target has nearly all the probability: the target's own entry, p - 1, is a difference of fp32
+    values next to 1, every other entry as small as its probability."""
+    x, w, b, t = _make(32, 48, 300, seed=23)
+    w[t] += 6.0 * x / x.square().sum(1, keepdim=True) * 4.0
+    _, grads = _run(x, w, b, t)
+    want = _want(x, w, b, t, 0.0)
+    for k, got in grads.items():
+        _close(got, want[k], k)
+
+
 @pytest.mark.parametrize("P,D,V", [(40, 32, 64), (64, 33, 50), (7, 2, 20), (300, 1, 9), (2, 3, 5)])
 @pytest.mark.parametrize("value", [1e6, 1e20, 3e38])
 def test_rows_that_do_not_count_may_hold_large_values(cuda, P, D, V, value):

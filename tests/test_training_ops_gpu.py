@@ -160,3 +160,48 @@ def test_token_losses_of_a_model(cuda):
     rows, mean = F.linear_token_losses(features, Value.leaf(model.head.weight.data), Value.leaf(model.head.bias.data), targets)
     assert rows.shape == targets.shape and float(rows[0, :5].abs().max()) == 0.0
     assert abs(float(mean) - float(model.loss(ids, targets).data)) <= 1e-6 * float(mean)
+
+
+def _first_step(fused, ids, targets, shards=4):
+    """(shard gradients by parameter name, flat shard gradients) of a trainer's first step."""
+    model = _model(CONFIGS[5], seed=11)
+    trainer = ShardedTrainer(model, nn.AdamW(model.parameters(), lr=1e-3), shards=shards, fused_loss=fused)
+    trainer.step(ids, targets)
+    names = [n for n, _ in model.named_parameters()]
+    return dict(zip(names, trainer.shard_grads.split(trainer.sizes, dim=1))), trainer.shard_grads
+
+
+def test_fused_loss_gradients_per_parameter(cuda):
+    """Each shard's gradient of each parameter, with and without the kept logits: both are within 1.6e-4 of the
+    exact one's largest entry (test_model_gradients), so within twice that of one another's (and 1.6e-4 of the
+    tolerance for taking the other form's entry as the size)."""
+    ids, targets = _batch(97)
+    fused, kept = (_first_step(f, ids, targets)[0] for f in (True, False))
+    for name, want in kept.items():
+        size = kept[name.replace(".k.", ".v.")] if name.endswith("attn.k.bias") else want
+        top = size.abs().amax(1)
+        assert torch.all(top > 0), name
+        assert torch.all((fused[name] - want).abs().amax(1) <= 3.3e-4 * top), name
+
+
+def test_fused_loss_shards_do_not_depend_on_one_another(cuda):
+    """A shard's gradients have the same bits whatever the other shards' rows are, and when the batch is split over
+    two ranks (two groups of a half batch each, as a rank runs them)."""
+    ids, targets = _batch(97)
+    _, want = _first_step(True, ids, targets)
+    other_ids, other_targets = _batch(97, seed=77)
+    for z in range(4):
+        rows = slice(2 * z, 2 * z + 2)
+        mixed, mixed_targets = other_ids.clone(), other_targets.clone()
+        mixed[rows], mixed_targets[rows] = ids[rows], targets[rows]
+        assert torch.equal(_first_step(True, mixed, mixed_targets)[1][z], want[z])
+    norm = torch.tensor([1.0 / ids.numel()], device="cuda")
+    for half in (0, 1):
+        model = _model(CONFIGS[5], seed=11)
+        for p in model.parameters():
+            p.grad, p.grad_fresh = torch.empty(2, p.data.numel(), device="cuda"), True
+        rows = slice(4 * half, 4 * half + 4)
+        with F.param_groups(2):
+            model.loss(ids[rows], targets[rows], grad_norm=norm).backward()
+        got = torch.cat([p.grad for p in model.parameters()], dim=1)
+        assert torch.equal(got, want[2 * half: 2 * half + 2])
