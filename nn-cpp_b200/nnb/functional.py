@@ -71,10 +71,12 @@ def _check_grouped(who: str, params) -> None:
     for p in params:
         if p is None or not p.requires_grad:
             continue
-        buf = p.data if p.grad is None or p.grad_borrowed else p.grad       # (grad_accum makes one like the data)
-        if (_GROUPS > 1 or buf.shape != p.data.shape) and not _holds_groups(buf, p.data.numel()):
+        n, buf = p.data.numel(), p.grad
+        if buf is None or p.grad_borrowed:               # grad_accum makes one like the data
+            buf = p.data
+        if (_GROUPS > 1 or buf.numel() != n) and not _holds_groups(buf, n):
             raise TensorShapeError(f"{who}: a gradient buffer of shape {tuple(buf.shape)} does not hold {_GROUPS} group(s) of "
-                                   f"{p.data.numel()} elements")
+                                   f"{n} elements")
 
 
 # ---- linear (ops.cpp:714-745) -------------------------------------------------------------------
@@ -421,9 +423,11 @@ def residual_norm(x: Value, branch: Value, gamma: Value, beta: Value | None = No
             raise TensorShapeError("residual_norm: the gate's rows do not divide into the parameter groups")
     if R % _GROUPS:
         raise TensorShapeError("residual_norm: the rows do not divide into the parameter groups")
-    params = [v for v in (gamma, beta, post_gamma, post_beta, gate if gate_rows == 1 else None) if v is not None and _need(v)]
-    if len({id(v) for v in params}) != len(params):
-        raise ValueError("residual_norm: one parameter in two places would share a gradient buffer")
+    params = (gamma, beta, post_gamma, post_beta, gate if gate_rows == 1 else None)
+    if post_gamma is not None or gate_rows == 1 or gamma is beta:
+        trained = [id(v) for v in params if v is not None and _need(v)]
+        if len(set(trained)) != len(trained):
+            raise ValueError("residual_norm: one parameter in two places would share a gradient buffer")
     _check_buffers("residual_norm", (x, branch, gamma, beta, post_gamma, post_beta, gate))
     k = NORM_LAYER if layer else NORM_RMS
     opt = lambda v: None if v is None else v.data.data_ptr()
