@@ -420,15 +420,17 @@ NNB_API nnb_status nnb_sequence_ce_bwd(void* stream, size_t P, size_t V, const f
  * ignore_index. The rows are processed in pieces: where gradients are wanted a piece's logits take at most
  * 512 MiB of scratch memory (or 128 rows), and become its gradient's packed form in place; w and the piece of
  * x have packed copies of their own size. Math mode NNB_MATH_FP32X3 splits the products' operands into two
- * fp16 parts after scaling them by a power of two (22 bits for values down to 2^-17 of the largest of w, of
- * the group's x or of a logit's gradient, 1; smaller ones to 2^-39 of it), NNB_MATH_TF32 keeps one part.
+ * fp16 parts after scaling every block of 128 x 128 of w, of a piece of x and of its logits' gradient by a power
+ * of two (22 bits for values down to 2^-17 of the block's largest, smaller ones to 2^-39 of it),
+ * NNB_MATH_TF32 keeps one part.
  * dx [P, D], dw [V, D], db [V] (each nullable; all NULL: no gradients are computed) receive the gradients
  * of the SUM of the row losses: the backward of the mean multiplies them by grad_loss * norm
  * (nnb_scaled_accumulate). dw and db are kept per group of P / groups consecutive rows, dw_stride and
  * db_stride apart (0: back to back), as nnb_linear_bwd_grouped's; a group's sums depend on its own rows
  * only. A row with a value of x that is not finite, or whose logits have no finite maximum (all -inf, +inf or
  * NaN), has loss and gradients NaN, and so has every row when w holds a value that is not finite; rows whose
- * target is ignore_index contribute nothing whatever they hold. */
+ * target is ignore_index contribute nothing whatever they hold (nor do those with an out-of-range target to dw
+ * and db). */
 NNB_API nnb_status nnb_linear_ce_fwd(void* stream, size_t P, size_t D, size_t V, size_t groups, const float* x,
 		const float* w, const float* bias, const int64_t* targets, int64_t ignore_index, float label_smoothing,
 		float* row_loss, float* loss, float* norm, float* dx, float* dw, size_t dw_stride, float* db, size_t db_stride);

@@ -13,8 +13,10 @@
 // backward pass would cost 8. The backward pass only scales the gradients by the upstream gradient over
 // the number of rows that count, which is known at the end.
 //
-// Ranges (split16): X and W are scaled by their largest magnitude, G by 2^15 (|G| <= 1): an entry of G below
-// 2^-17 loses relative precision, down to an absolute 2^-40, next to the -1 of its row's target.
+// Ranges (split16): blocks of 128 x 128 of X, W and G are scaled by their largest magnitude. An entry of G below
+// 2^-17 of its block's largest loses relative precision, down to an absolute 2^-40 where the block holds a target
+// (whose entry, softmax - 1, is at most 1): a token that is nobody's target and has probabilities near 2^-40 keeps
+// few bits in its row of dW where other tokens of its block are targets.
 #include <algorithm>
 #include <cmath>
 
@@ -33,7 +35,6 @@ using split16::kRows;
 
 constexpr size_t kPieceBytes = size_t(512) << 20;   // G (and the logits before it) of one piece
 constexpr size_t kPartBytes = size_t(256) << 20;    // softmax statistics of one piece
-constexpr int kGShift = 15;                         // G is packed times 2^15
 constexpr float kLog2e = 1.44269504088896341f;
 
 // What the gradient needs of a row.
@@ -47,7 +48,7 @@ struct RowInfo {
 // loss and RowInfo.
 __global__ void __launch_bounds__(256) ce_rows_kernel(const float2* part, const float* part_sum,
 		const float* target_logit, int parts, int rows, int rows_pad, int V, const int64_t* targets,
-		int64_t ignore_index, float ls, const int* x_bad, const split16::Range* w_range,
+		int64_t ignore_index, float ls, const int* x_bad, const int* w_bad,
 		float* row_loss, int* valid, RowInfo* info, int* err) {
 	__shared__ float2 ms[32][9];
 	__shared__ float tot[32][9];
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const float2* part, const 
 			if (t != ignore_index) atomicCAS(err, 0, kDevBadIndex);
 		} else {
 			// no finite maximum, or a value of x or w that is not finite (packed as zero): NaN
-			if (!(top > -INFINITY && top < INFINITY) || x_bad[r] || w_range->bad) sum = __int_as_float(0x7fc00000);
+			if (!(top > -INFINITY && top < INFINITY) || x_bad[r] || *w_bad) sum = __int_as_float(0x7fc00000);
 			const float lse = logf(sum), nll = lse - (target_logit[r] - top);
 			row_loss[r] = ls == 0.0f ? nll : (1.0f - ls) * nll + ls * (lse - (total / (float)V - top));
 			valid[r] = 1;
@@ -105,33 +106,39 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 	return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One block of 128 rows x 64 columns per CTA, in place: logits in, G out as fp16 parts; its column sums.
-// A thread holds four columns of eight rows. HBM bound: 4 bytes in and 4 out per logit (185 us for 134 M
-// logits, 5.8 TB/s).
-__global__ void __launch_bounds__(256) ce_grad_kernel(float* blocks, int kw, int V, int rows_pad,
-		const RowInfo* info, float ls, int two_parts, float* col_part) {
-	__shared__ float4 sums[8][16];
-	const int c64 = blockIdx.x, rb = blockIdx.y, tid = threadIdx.x, q = tid & 15, r0 = tid >> 4;
+// One block of 128 x 128 per CTA (two packed blocks of 64 columns, or the last one), in place: logits in, G out as
+// fp16 parts with the block's scale; its column sums. A warp holds 128 columns of eight rows, four per lane. HBM
+// bound: 4 bytes in and 4 out per logit (196 us for 134 M logits, 5.5 TB/s).
+__global__ void __launch_bounds__(512, 2) ce_grad_kernel(float* blocks, int kw, int V, const RowInfo* info, float ls,
+		int two_parts, int* shifts, float* col_part) {
+	__shared__ RowInfo rows[kRows];
+	__shared__ float4 sums[16][32];
+	__shared__ unsigned tops[16];
+	const int rb = blockIdx.y, tid = threadIdx.x, q = tid & 31, r0 = tid >> 5, c64 = blockIdx.x * 2 + (q >> 4);
+	const bool in = c64 < kw;
 	float* block = blocks + ((long long)rb * kw + c64) * (kRows * kCols);
-	const int col = c64 * kCols + q * 4;
-	const float spread = ls / (float)V, scale = exp2f((float)kGShift);
+	const int col = blockIdx.x * 2 * kCols + q * 4;
+	const float spread = ls / (float)V;
 	chain_wait();
 	float4 l[8];
-	RowInfo in[8];
 #pragma unroll
-	for (int i = 0; i < 8; ++i) {
-		l[i] = reinterpret_cast<const float4*>(block)[(r0 + 16 * i) * (kCols / 4) + q];
-		in[i] = info[rb * kRows + r0 + 16 * i];
-	}
+	for (int i = 0; i < 8; ++i)
+		l[i] = in ? reinterpret_cast<const float4*>(block)[(r0 + 16 * i) * (kCols / 4) + (q & 15)] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+	if (tid < kRows) rows[tid] = info[rb * kRows + tid];
+	__syncthreads();
 	float4 cs = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+	unsigned top = 0;
 #pragma unroll
 	for (int i = 0; i < 8; ++i) {
+		const RowInfo row = rows[r0 + 16 * i];
 		float g[4] = {l[i].x, l[i].y, l[i].z, l[i].w};
 #pragma unroll
 		for (int k = 0; k < 4; ++k) {
-			float v = exp2_hw((g[k] - in[i].top) * kLog2e) * in[i].inv - spread;
-			if (col + k == in[i].target) v -= 1.0f - ls;
-			g[k] = in[i].target >= 0 && col + k < V ? v : 0.0f;
+			float v = exp2_hw((g[k] - row.top) * kLog2e) * row.inv - spread;
+			if (col + k == row.target) v -= 1.0f - ls;
+			g[k] = row.target >= 0 && col + k < V ? v : 0.0f;
+			const unsigned bits = __float_as_uint(g[k]) & 0x7fffffffu;
+			if (bits < 0x7f800000u) top = max(top, bits);          // (a NaN row stays NaN at any scale)
 		}
 		l[i] = make_float4(g[0], g[1], g[2], g[3]);
 		cs.x += g[0];
@@ -139,35 +146,42 @@ __global__ void __launch_bounds__(256) ce_grad_kernel(float* blocks, int kw, int
 		cs.z += g[2];
 		cs.w += g[3];
 	}
+	top = __reduce_max_sync(0xffffffffu, top);
+	if (q == 0) tops[r0] = top;
+	sums[r0][q] = cs;
 	__syncthreads();                               // every logit of the block is in registers
-	unsigned char* out = reinterpret_cast<unsigned char*>(block);
 #pragma unroll
-	for (int i = 0; i < 8; ++i) {
-		const float4 v = make_float4(l[i].x * scale, l[i].y * scale, l[i].z * scale, l[i].w * scale);
-		const uint2 hi = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
-		unsigned char* dst = out + (r0 + 16 * i) * (kCols * 2) + q * 8;
-		*reinterpret_cast<uint2*>(dst) = hi;
-		if (two_parts) {
-			const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)),
-				h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-			*reinterpret_cast<uint2*>(dst + split16::kPartBytes) =
-				make_uint2(half2_bits(v.x - h0.x, v.y - h0.y), half2_bits(v.z - h1.x, v.w - h1.y));
+	for (int k = 0; k < 16; ++k) top = max(top, tops[k]);
+	const int shift = split16::block_shift(top);
+	const float scale = split16::exp2_int(shift);
+	if (tid == 0) shifts[rb * gridDim.x + blockIdx.x] = shift;
+	if (in) {
+		unsigned char* out = reinterpret_cast<unsigned char*>(block);
+#pragma unroll
+		for (int i = 0; i < 8; ++i) {
+			const float4 v = make_float4(l[i].x * scale, l[i].y * scale, l[i].z * scale, l[i].w * scale);
+			const uint2 hi = make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
+			unsigned char* dst = out + (r0 + 16 * i) * (kCols * 2) + (q & 15) * 8;
+			*reinterpret_cast<uint2*>(dst) = hi;
+			if (two_parts) {
+				const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)),
+					h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+				*reinterpret_cast<uint2*>(dst + split16::kPartBytes) =
+					make_uint2(half2_bits(v.x - h0.x, v.y - h0.y), half2_bits(v.z - h1.x, v.w - h1.y));
+			}
 		}
 	}
-	if (!col_part) return;
-	// rows r0 and r0 + 1 of a warp, then the eight warps in order
-	cs.x += __shfl_xor_sync(0xffffffffu, cs.x, 16);
-	cs.y += __shfl_xor_sync(0xffffffffu, cs.y, 16);
-	cs.z += __shfl_xor_sync(0xffffffffu, cs.z, 16);
-	cs.w += __shfl_xor_sync(0xffffffffu, cs.w, 16);
-	if ((tid & 31) < 16) sums[tid >> 5][q] = cs;
-	__syncthreads();
-	if (tid >= 64) return;
+	if (!col_part || tid >= kRows || blockIdx.x * kRows + tid >= kw * kCols) return;
+	// the sixteen warps' sums, in pairs
 	const float* f = reinterpret_cast<const float*>(sums);
-	float s = f[tid];
+	float s[16];
 #pragma unroll
-	for (int k = 1; k < 8; ++k) s += f[k * 64 + tid];
-	col_part[(long long)rb * kw * kCols + c64 * kCols + tid] = s;
+	for (int k = 0; k < 16; ++k) s[k] = f[k * kRows + tid];
+#pragma unroll
+	for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+		for (int k = 0; k < o; ++k) s[k] += s[k + o];
+	col_part[(long long)rb * kw * kCols + blockIdx.x * kRows + tid] = s[0];
 }
 
 // db (+)= the row blocks' column sums: 32 columns per CTA, warp y sums blocks y, y + 8, ..., then the eight
@@ -292,7 +306,7 @@ struct Scratch {
 struct Layout {
 	long long piece, blocks;                  // rows of a piece, and their 128-row blocks
 	int dx_splits, dw_splits;                 // depth splits of the gradients' products
-	size_t ranges, wpack, xpack, x_bad, g, part, part_sum, target_logit, info, losses, valid, cols, slabs;
+	size_t flags, wpack, wshift, xpack, xshift, g, gshift, part, part_sum, target_logit, info, losses, valid, cols, slabs;
 };
 
 Layout plan(const Call& c, Scratch& s) {
@@ -302,13 +316,13 @@ Layout plan(const Call& c, Scratch& s) {
 	const size_t pad = (size_t)l.blocks * kRows;
 	l.dx_splits = c.dx ? split16::choose_splits(l.piece, c.D, c.V) : 1;
 	l.dw_splits = c.dw ? split16::choose_splits(c.V, c.D, l.piece) : 1;
-	// a range per group of x (a group's results depend on its own rows only) and w's, and x_bad: zeroed together
-	const size_t ranges = (size_t)(c.groups + 1) * sizeof(split16::Range);
-	l.ranges = s.take(ranges + (size_t)c.P * sizeof(int));
-	l.x_bad = l.ranges + ranges;
+	l.flags = s.take((size_t)(1 + c.P) * sizeof(int));         // w's values that are not finite, and each row of x's
 	l.wpack = s.take(split16::pack_bytes(c.V, c.D));
+	l.wshift = s.take(split16::shift_bytes(c.V, c.D));
 	l.xpack = s.take(split16::pack_bytes(l.piece, c.D));
+	l.xshift = s.take(split16::shift_bytes(l.piece, c.D));
 	l.g = s.take(c.grad() ? (size_t)l.blocks * c.kw() * kBlockBytes : 0);
+	l.gshift = s.take(c.grad() ? split16::shift_bytes(l.piece, c.V) : 0);
 	l.part = s.take((size_t)c.parts() * pad * sizeof(float2));
 	l.part_sum = s.take(c.ls != 0.0f ? (size_t)c.parts() * pad * sizeof(float) : 0);
 	l.target_logit = s.take(pad * sizeof(float));
@@ -323,31 +337,26 @@ Layout plan(const Call& c, Scratch& s) {
 
 nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l, const Scratch& m) {
 	const int parts = math_mode() == NNB_MATH_FP32X3 ? 2 : 1;
-	split16::Range* ranges = m.at<split16::Range>(l.ranges);
-	const split16::Range* wr = ranges + c.groups;
+	int* w_bad = m.at<int>(l.flags);
 	float* row_loss = c.row_loss ? c.row_loss : m.at<float>(l.losses);
 	int* valid = m.at<int>(l.valid);
 	const long long rg = c.P / c.groups;             // parameter gradients are kept per group of rows
-	NNB_CUDA_TRY(cudaMemsetAsync(ranges, 0, (size_t)(c.groups + 1) * sizeof(split16::Range) + (size_t)c.P * sizeof(int), s));
-	const split16::LiveRows live{c.targets, c.ignore_index, c.V};
-	NNB_TRY(split16::find_ranges(s, c.x, rg, c.D, c.groups, live, c.w, c.V * c.D, ranges));
+	NNB_CUDA_TRY(cudaMemsetAsync(w_bad, 0, (size_t)(1 + c.P) * sizeof(int), s));
 	split16::Pack W, X, G;
-	W.buf = m.at<void>(l.wpack); W.rows = c.V; W.cols = c.D;
+	W.buf = m.at<void>(l.wpack); W.shift = m.at<int>(l.wshift); W.rows = c.V; W.cols = c.D;
 	for (long long z = 0; z < c.groups; ++z) {
 		for (long long r0 = z * rg; r0 < (z + 1) * rg;) {
 			const long long n = std::min(l.piece, (z + 1) * rg - r0), blocks = (n + kRows - 1) / kRows, pad = blocks * kRows;
 			const int first = r0 == z * rg;
-			const split16::Range* xr = ranges + z;
 			const float* x = c.x + r0 * c.D;
-			int* x_bad = m.at<int>(l.x_bad) + r0;
+			int* x_bad = w_bad + 1 + r0;
 			const split16::PackJob jobs[2] = {
-				{x, n, c.D, blocks, xr, m.at<void>(l.xpack), x_bad, {c.targets + r0, c.ignore_index, c.V}},
-				{c.w, c.V, c.D, (c.V + 2 * kRows - 1) / (2 * kRows) * 2, wr, m.at<void>(l.wpack), nullptr, {}}};
+				{x, n, c.D, blocks, m.at<void>(l.xpack), m.at<int>(l.xshift), x_bad, 1, {c.targets + r0, c.ignore_index, c.V}},
+				{c.w, c.V, c.D, split16::even_blocks(c.V), m.at<void>(l.wpack), m.at<int>(l.wshift), w_bad, 0, {}}};
 			NNB_TRY(split16::pack(s, jobs, r0 == 0 ? 2 : 1, parts));           // W with the first piece
-			X.buf = m.at<void>(l.xpack); X.rows = n; X.cols = c.D;
+			X.buf = m.at<void>(l.xpack); X.shift = m.at<int>(l.xshift); X.rows = n; X.cols = c.D;
 
 			split16::Product p;
-			p.ra = xr; p.rb = wr;
 			p.bias = c.bias;
 			p.targets = c.targets + r0;
 			p.part = m.at<float2>(l.part);
@@ -362,28 +371,27 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 			{
 				TraceScope ts(s, kTraceRowwise);
 				NNB_CUDA_TRY(launch_chained(ce_rows_kernel, (unsigned)(pad / 8), 256, 0, s, p.part, p.part_sum, p.target_logit,
-					(int)c.parts(), (int)n, (int)pad, (int)c.V, p.targets, c.ignore_index, c.ls, x_bad, wr, row_loss + r0,
+					(int)c.parts(), (int)n, (int)pad, (int)c.V, p.targets, c.ignore_index, c.ls, x_bad, w_bad, row_loss + r0,
 					valid + r0, info, dev->error_word));
 			}
 			if (c.grad()) {
 				float* cols = c.db ? m.at<float>(l.cols) : nullptr;
 				{
 					TraceScope ts(s, kTraceRowwise);
-					NNB_CUDA_TRY(launch_chained(ce_grad_kernel, dim3((unsigned)c.kw(), (unsigned)blocks), 256, 0, s, p.blocks,
-						(int)c.kw(), (int)c.V, (int)pad, info, c.ls, (int)(parts == 2), cols));
+					NNB_CUDA_TRY(launch_chained(ce_grad_kernel, dim3((unsigned)((c.kw() + 1) / 2), (unsigned)blocks), 512, 0, s,
+						p.blocks, (int)c.kw(), (int)c.V, info, c.ls, (int)(parts == 2), m.at<int>(l.gshift), cols));
 				}
 				if (c.db) {
 					TraceScope ts(s, kTraceRowwise);
 					NNB_CUDA_TRY(launch_chained(ce_bias_kernel, (unsigned)((c.V + 31) / 32), 256, 0, s, cols, (int)blocks,
 						(int)(c.kw() * kCols), (int)c.V, c.db + z * c.db_stride, first));
 				}
-				G.buf = m.at<void>(l.g); G.rows = n; G.cols = c.V;
+				G.buf = m.at<void>(l.g); G.shift = m.at<int>(l.gshift); G.rows = n; G.cols = c.V;
 			}
 			// a product cut along its depth leaves its pieces in slabs, summed in order
-			auto product = [&](const split16::Pack& a, bool mn_a, const split16::Pack& b, const split16::Range* rb, long long M,
+			auto product = [&](const split16::Pack& a, bool mn_a, const split16::Pack& b, long long M,
 					long long K, int max_splits, float* out, int accumulate) -> nnb_status {
 				split16::Product d;
-				d.rb = rb; d.shift = kGShift;
 				d.splits = split16::split_count(K, std::min(max_splits, split16::choose_splits(M, c.D, K)));
 				const bool cut = d.splits > 1;
 				d.C = cut ? m.at<float>(l.slabs) : out;
@@ -392,8 +400,8 @@ nnb_status run(cudaStream_t s, const Call& c, DeviceState* dev, const Layout& l,
 				NNB_TRY(split16::run(s, d, split16::kStore, parts, a, mn_a, b, true, M, c.D, K));
 				return cut ? split16::sum_slabs(s, d.C, d.splits, M * c.D, out, accumulate) : NNB_OK;
 			};
-			if (c.dx) NNB_TRY(product(G, false, W, wr, n, c.V, l.dx_splits, c.dx + r0 * c.D, 0));                        // G W
-			if (c.dw) NNB_TRY(product(G, true, X, xr, c.V, n, l.dw_splits, c.dw + z * c.dw_stride, !first));             // G^T X
+			if (c.dx) NNB_TRY(product(G, false, W, n, c.V, l.dx_splits, c.dx + r0 * c.D, 0));                        // G W
+			if (c.dw) NNB_TRY(product(G, true, X, c.V, n, l.dw_splits, c.dw + z * c.dw_stride, !first));             // G^T X
 			r0 += n;
 		}
 	}

@@ -1,10 +1,10 @@
-// split16.cu -- the fp16-split product (nnb_split16.cuh): range, pack and the tcgen05 kernel.
+// split16.cu -- the fp16-split product (nnb_split16.cuh): pack and the tcgen05 kernel.
 //
 // The kernel is warp-specialised, one CTA per SM, 12 warps:
 //   warp 0     TMA producer: a stage holds a 32-deep k-block, A 128 and B 256 rows (or columns), hi[, lo];
 //   warp 1     MMA issuer: kind::f16 128 x 256 x 16 into two TMEM accumulators in turn, one accumulator per
 //              chunk of 128 terms (3 x 8 MMAs);
-//   warps 4-11 epilogue: add each finished chunk into registers (128 columns per thread) while the tensor
+//   warps 4-11 epilogue: add each finished chunk, scaled back, into registers (128 columns per thread) while the tensor
 //              core works on the next, then store or reduce.
 // The 384 threads are launched with 168 registers each; warps 0-3 hand theirs down to 56 and the epilogue
 // takes 224 (4 x 32 x 56 + 8 x 32 x 224 = 384 x 168), which hold the 128 sums.
@@ -27,69 +27,7 @@ namespace split16 {
 
 namespace {
 
-// ---- range and pack --------------------------------------------------------------------------
-
-struct RangeJobs {
-	const float *x, *w;
-	long long rows, cols, n, nw;               // of each group of x (n = rows cols), and of w
-	int vec, vec_w, groups;
-	LiveRows live;
-	Range* out;
-};
-
-// grid.y: the groups of x, then w. A value of x counts if its row does.
-__global__ void __launch_bounds__(256) range_kernel(const RangeJobs jobs) {
-	const bool is_w = (int)blockIdx.y == jobs.groups;
-	const float* x = is_w ? jobs.w : jobs.x + blockIdx.y * jobs.n;
-	const long long n = is_w ? jobs.nw : jobs.n, cols = jobs.cols, row0 = blockIdx.y * jobs.rows;
-	const int vec = is_w ? jobs.vec_w : jobs.vec;
-	const bool all = is_w || !jobs.live.targets;
-	Range* out = jobs.out + blockIdx.y;
-	chain_wait();
-	unsigned top = 0, bad = 0;
-	auto see = [&](float v) {
-		const unsigned b = __float_as_uint(v) & 0x7fffffffu;
-		if (b >= 0x7f800000u) bad = 1;
-		else top = max(top, b);
-	};
-	auto row_of = [&](long long e) { return n < 0x7fffffffLL ? (long long)((unsigned)e / (unsigned)cols) : e / cols; };
-	const long long step = (long long)gridDim.x * blockDim.x;
-	long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
-	if (vec) {
-		const float4* x4 = reinterpret_cast<const float4*>(x);
-#pragma unroll 4
-		for (; i < n / 4; i += step) {
-			const float4 v = x4[i];
-			if (!all) {
-				const long long r = row_of(4 * i);
-				if (4 * i + 3 - r * cols >= cols) {          // these four lie in several rows
-					const float q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-					for (int k = 0; k < 4; ++k)
-						if (jobs.live(row0 + row_of(4 * i + k))) see(q[k]);
-					continue;
-				}
-				if (!jobs.live(row0 + r)) continue;
-			}
-			see(v.x);
-			see(v.y);
-			see(v.z);
-			see(v.w);
-		}
-	} else {
-#pragma unroll 4
-		for (; i < n; i += step) {
-			const float v = x[i];
-			if (all || jobs.live(row0 + row_of(i))) see(v);
-		}
-	}
-	top = __reduce_max_sync(0xffffffffu, top);
-	bad = __reduce_or_sync(0xffffffffu, bad);
-	if ((threadIdx.x & 31) == 0) {                 // a maximum: the order does not matter
-		if (top) atomicMax(&out->top, top);
-		if (bad) atomicOr(&out->bad, 1u);
-	}
-}
+// ---- pack ------------------------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 	const __half2 h = __floats2half2_rn(a, b);
@@ -98,68 +36,86 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 struct PackWork {
 	const float* x;
-	long long rows, cols, total;               // total: quads of the padded matrix
-	int vec;
-	const Range* range;
+	long long rows, cols;
+	int kw, scale_cols, vec;
 	unsigned char* out;
-	int* row_bad;
+	int* shift;
+	int* bad;
+	int per_row;
 	LiveRows live;
 };
 struct PackJobs {
 	PackWork job[2];
+	int first;                                 // CTAs of job 0
 	int parts;
 };
 
-// Four columns per thread: a float4 in (or four floats), 8 bytes of hi and of lo out. grid.y: the matrix.
-__global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
-	const PackWork& w = jobs.job[blockIdx.y];
-	const float* x = w.x;
-	unsigned char* out = w.out;
-	int* row_bad = w.row_bad;
-	const long long rows = w.rows, cols = w.cols, total = w.total;
-	const int vec = w.vec, parts = jobs.parts;
+// One block of 128 x 128 per CTA, held in registers: 16 float4 per thread (or single floats), a warp on the 128
+// columns of a row; its largest magnitude; then 8 bytes of hi and of lo out per float4. HBM bound: 4 bytes in and
+// 4 out per value (131072 x 512: 97 us, 5.5 TB/s; a range pass over the matrix and a pack after it took 148).
+__global__ void __launch_bounds__(256, 2) pack_kernel(const PackJobs jobs) {
+	__shared__ unsigned tops[8];
+	const bool second = (int)blockIdx.x >= jobs.first;
+	const PackWork& w = jobs.job[second];
+	const int b = (int)blockIdx.x - (second ? jobs.first : 0), rb = b / w.scale_cols, cb = b - rb * w.scale_cols;
+	const int q = threadIdx.x & 31, r0 = threadIdx.x >> 5;
+	const long long cols = w.cols, c = cb * (long long)kRows + q * 4, row0 = rb * (long long)kRows;
 	chain_wait();
-	const float s = exp2_int(range_shift(w.range));
-	const long long kw = (cols + kCols - 1) / kCols, quads = kw * (kCols / 4);
-	for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-		long long r, q;
-		if (total < 0x7fffffffLL) {
-			r = (unsigned)i / (unsigned)quads;
-			q = (unsigned)i - (unsigned)r * (unsigned)quads;
-		} else {
-			r = i / quads;
-			q = i - r * quads;
-		}
-		const long long c = q * 4;
-		float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-		if (r < rows && c < cols && w.live(r)) {
-			const float* src = x + r * cols + c;
-			if (vec) {
+	float v[16][4];
+#pragma unroll
+	for (int i = 0; i < 16; ++i) {
+		const long long r = row0 + r0 + 8 * i;
+		v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+		if (r < w.rows && c < cols) {
+			const float* src = w.x + r * cols + c;
+			if (w.vec) {
 				const float4 t = *reinterpret_cast<const float4*>(src);
-				v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+				v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
 			} else {
 #pragma unroll
 				for (int k = 0; k < 4; ++k)
-					if (c + k < cols) v[k] = src[k];
+					if (c + k < cols) v[i][k] = src[k];
 			}
 		}
+	}
+	unsigned top = 0;
+#pragma unroll
+	for (int i = 0; i < 16; ++i) {
+		const long long r = row0 + r0 + 8 * i;
+		const bool live = r < w.rows && w.live(r);
 		bool bad = false;
+#pragma unroll
+		for (int k = 0; k < 4; ++k) {
+			const unsigned bits = __float_as_uint(v[i][k]) & 0x7fffffffu;
+			bad |= bits >= 0x7f800000u;
+			if (!live || bits >= 0x7f800000u) v[i][k] = 0.0f;
+			else top = max(top, bits);
+		}
+		if (live && bad) w.bad[w.per_row ? r : 0] = 1;       // every writer writes 1
+	}
+	top = __reduce_max_sync(0xffffffffu, top);
+	if (q == 0) tops[r0] = top;
+	__syncthreads();
+#pragma unroll
+	for (int k = 0; k < 8; ++k) top = max(top, tops[k]);
+	const int shift = block_shift(top);
+	if (threadIdx.x == 0) w.shift[b] = shift;
+	const int c64 = 2 * cb + (q >> 4);
+	if (c64 >= w.kw) return;
+	const float s = exp2_int(shift);
+	unsigned char* dst = w.out + (rb * (long long)w.kw + c64) * kBlockBytes + r0 * (kCols * 2) + (q & 15) * 8;
+#pragma unroll
+	for (int i = 0; i < 16; ++i, dst += 8 * kCols * 2) {
 		float hi[4];
 #pragma unroll
 		for (int k = 0; k < 4; ++k) {
-			if (!isfinite(v[k])) {
-				bad = true;
-				v[k] = 0.0f;
-			}
-			v[k] *= s;
-			hi[k] = __half2float(__float2half_rn(v[k]));
+			v[i][k] *= s;
+			hi[k] = __half2float(__float2half_rn(v[i][k]));
 		}
-		if (bad && row_bad) row_bad[r] = 1;            // every writer writes 1
-		unsigned char* dst = out + ((r >> 7) * kw + (c >> 6)) * kBlockBytes + (r & 127) * (kCols * 2) + (c & 63) * 2;
 		*reinterpret_cast<uint2*>(dst) = make_uint2(half2_bits(hi[0], hi[1]), half2_bits(hi[2], hi[3]));
-		if (parts == 2)
-			*reinterpret_cast<uint2*>(dst + kPartBytes) =
-				make_uint2(half2_bits(v[0] - hi[0], v[1] - hi[1]), half2_bits(v[2] - hi[2], v[3] - hi[3]));
+		if (jobs.parts == 2)
+			*reinterpret_cast<uint2*>(dst + kPartBytes) = make_uint2(half2_bits(v[i][0] - hi[0], v[i][1] - hi[1]),
+				half2_bits(v[i][2] - hi[2], v[i][3] - hi[3]));
 	}
 }
 
@@ -367,10 +323,6 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 		const int row = quad * 32 + lane;
 		float* stage = reinterpret_cast<float*>(smem + (size_t)kStages * kStageBytes + (warp - 4) * kEpiTile);
 		float4* st4 = reinterpret_cast<float4*>(stage);
-		// acc is scaled back by 2^e: in one factor, or two where the exponent does not fit one
-		const int e = -p.shift - (p.ra ? range_shift(p.ra) : 0) - (p.rb ? range_shift(p.rb) : 0);
-		const int e1 = max(-126, min(127, e)), e2 = max(-126, min(127, e - e1));
-		const float alpha = exp2_int(e1), alpha2 = exp2_int(e2);
 		const bool vec_ok = kEpi == kStore && p.ldc % 4 == 0 && p.slab % 4 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15) == 0;
 		int v = 0;
 		bool ok = true;
@@ -379,7 +331,15 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 			float2 acc[kBN / 4];                           // this thread's row, 128 columns in pairs
 #pragma unroll
 			for (int j = 0; j < kBN / 4; ++j) acc[j] = make_float2(0.0f, 0.0f);
+			const int nb = min(it.nt * 2 + half, p.b_last);      // (past the last block there are zeros, whatever their scale)
 			for (int c0 = it.kb0; c0 < it.kb1; c0 += kChunkKb, ++v) {
+				// the chunk's terms are scaled back by 2^e: in one factor, or two where the exponent does not fit one.
+				// (The loads' latency passes in the wait.)
+				const int kc = c0 / kChunkKb;
+				const int e = -p.sa[kMnA ? kc * p.a_sw + it.mt : it.mt * p.a_sw + kc] -
+					p.sb[kMnB ? kc * p.b_sw + nb : nb * p.b_sw + kc];
+				const int e1 = max(-126, min(127, e));
+				const float2 back = make_float2(exp2_int(e1), exp2_int(e1));
 				if (!mbar_wait_warp(smem_u32(&accf_bar[v & 1]), (v >> 1) & 1, p.err, kDevTimeoutAccum, abort_flag)) {
 					ok = false;
 					break;
@@ -391,9 +351,14 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 					uint32_t r[32];
 					tmem_ld_32x32b_x32(src + c * 32, r);
 					tmem_wait_ld();
+					if (e != e1) {                             // operands beyond 2^110 or below 2^-95: warp-uniform
+						const float more = exp2_int(e - e1);
+#pragma unroll
+						for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * more);
+					}
 #pragma unroll
 					for (int j = 0; j < 16; ++j)
-						acc[c * 16 + j] = add2_rn(acc[c * 16 + j], make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+						acc[c * 16 + j] = fma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), back, acc[c * 16 + j]);
 				}
 				tc_fence_before();
 				__syncwarp();
@@ -425,15 +390,9 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 				}
 				__syncwarp();
 			};
-			if (alpha2 != 1.0f) {
-#pragma unroll
-				for (int j = 0; j < kBN / 4; ++j) acc[j] = mul2_rn(acc[j], make_float2(alpha2, alpha2));
-			}
 			const int warp_row = it.mt * kBM + quad * 32, rows_here = max(0, min(32, p.M - warp_row));
 			if (kEpi == kStore) {
 				float* C = p.C + it.split * p.slab;
-#pragma unroll
-				for (int j = 0; j < kBN / 4; ++j) acc[j] = mul2_rn(acc[j], make_float2(alpha, alpha));
 #pragma unroll
 				for (int c = 0; c < kBN / 64; ++c) {
 					const int gn = n0 + c * 32;
@@ -450,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 					}
 				}
 			} else {
-				// l = acc 2^e + bias: the biases of the warp's 128 columns through its staging tile (one coalesced
+				// l = acc + bias: the biases of the warp's 128 columns through its staging tile (one coalesced
 				// load, then broadcasts)
 				if (p.bias) {
 					float4 b;
@@ -463,13 +422,10 @@ __global__ void __launch_bounds__(kThreads, 1) split16_kernel(const __grid_const
 #pragma unroll
 					for (int j = 0; j < kBN / 8; ++j) {
 						const float4 bj = st4[j];
-						acc[2 * j] = fma2_rn(acc[2 * j], make_float2(alpha, alpha), make_float2(bj.x, bj.y));
-						acc[2 * j + 1] = fma2_rn(acc[2 * j + 1], make_float2(alpha, alpha), make_float2(bj.z, bj.w));
+						acc[2 * j] = add2_rn(acc[2 * j], make_float2(bj.x, bj.y));
+						acc[2 * j + 1] = add2_rn(acc[2 * j + 1], make_float2(bj.z, bj.w));
 					}
 					__syncwarp();                          // read before the tile is written again
-				} else {
-#pragma unroll
-					for (int j = 0; j < kBN / 4; ++j) acc[j] = mul2_rn(acc[j], make_float2(alpha, alpha));
 				}
 				const long long slot = (long long)(it.nt * 2 + half) * (p.tiles_m * kBM) + gm;
 				if (p.part_sum) {
@@ -611,40 +567,24 @@ nnb_status dispatch(cudaStream_t s, const DeviceState* dev, int epilogue, bool m
 
 }  // namespace
 
-nnb_status find_ranges(cudaStream_t s, const float* x, long long rows, long long cols, long long groups, LiveRows live,
-		const float* w, long long nw, Range* out) {
-	const long long n = rows * cols;
-	RangeJobs jobs;
-	jobs.x = x; jobs.rows = rows; jobs.cols = cols; jobs.n = n; jobs.groups = (int)groups; jobs.live = live;
-	jobs.w = w; jobs.nw = nw; jobs.out = out;
-	jobs.vec = n % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-	jobs.vec_w = nw % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
-	const long long most = std::max(n, nw);
-	{
-		TraceScope ts(s, kTracePack);
-		NNB_CUDA_TRY(launch_chained(range_kernel, dim3((unsigned)std::min<long long>((most + 4095) / 4096, 148 * 8),
-			(unsigned)(groups + 1)), 256, 0, s, jobs));
-	}
-	return NNB_OK;
-}
-
 nnb_status pack(cudaStream_t s, const PackJob* jobs, int count, int parts) {
 	PackJobs k;
 	k.parts = parts;
-	long long most = 0;
+	long long ctas[2] = {0, 0};
 	for (int i = 0; i < count; ++i) {
 		const PackJob& j = jobs[i];
 		PackWork& w = k.job[i];
-		w.x = j.x; w.rows = j.rows; w.cols = j.cols; w.range = j.range;
-		w.out = static_cast<unsigned char*>(j.buf); w.row_bad = j.row_bad; w.live = j.live;
-		w.total = j.row_blocks * kRows * ((j.cols + kCols - 1) / kCols) * (kCols / 4);
+		w.x = j.x; w.rows = j.rows; w.cols = j.cols; w.live = j.live;
+		w.kw = (int)((j.cols + kCols - 1) / kCols); w.scale_cols = (int)((j.cols + kRows - 1) / kRows);
+		w.out = static_cast<unsigned char*>(j.buf); w.shift = j.shift; w.bad = j.bad; w.per_row = j.per_row;
 		w.vec = j.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(j.x) & 15) == 0;
-		most = std::max(most, w.total);
+		ctas[i] = j.row_blocks * w.scale_cols;
 	}
+	if (ctas[0] + ctas[1] > INT32_MAX) return fail(NNB_ERR_UNSUPPORTED, "split product: operand too large");
+	k.first = (int)ctas[0];
 	{
 		TraceScope ts(s, kTracePack);
-		NNB_CUDA_TRY(launch_chained(pack_kernel, dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 32), (unsigned)count),
-			256, 0, s, k));
+		NNB_CUDA_TRY(launch_chained(pack_kernel, (unsigned)(ctas[0] + ctas[1]), 256, 0, s, k));
 	}
 	return NNB_OK;
 }
@@ -692,6 +632,11 @@ nnb_status run(cudaStream_t s, Product p, int epilogue, int parts, const Pack& a
 	if ((p.kb + p.split_kb - 1) / p.split_kb != p.splits) return fail(NNB_ERR_INVALID, "split product: empty depth split");
 	p.a_kw = (int)a.kw();
 	p.b_kw = (int)b.kw();
+	p.sa = a.shift;
+	p.sb = b.shift;
+	p.a_sw = (int)a.scale_cols();
+	p.b_sw = (int)b.scale_cols();
+	p.b_last = (int)(mn_b ? b.scale_cols() : b.row_blocks()) - 1;
 	p.err = dev->error_word;
 	CUtensorMap ta, tb;
 	if (mn_a) NNB_TRY(map_mn(&ta, a, kBM / kCols));

@@ -343,6 +343,46 @@ def test_gradients_of_confident_rows(cuda):
         _close(got, want[k], k)
 
 
+def test_a_large_row_costs_the_others_no_bits(cuda):
+    """Operands are scaled by blocks of 128 rows: a row 2^40 times larger leaves the bits of the rows in other
+    blocks, their losses and their gradients, as they were."""
+    x, w, b, t = _make(400, 40, 300, seed=24)
+    x2 = x.clone()
+    x2[130] *= 2.0 ** 40
+    keep = [i for i in range(400) if not 128 <= i < 256]
+    norm = torch.tensor([1.0], device="cuda")
+    rows, grads = [], []
+    for data in (x, x2):
+        rows.append(F.linear_token_losses(*[Value.leaf(v, False) for v in (data, w, b)], t)[0])
+        grads.append(_run(data, w, b, t, grad_norm=norm)[1]["x"])
+    assert torch.equal(rows[0][keep], rows[1][keep]) and torch.equal(grads[0][keep], grads[1][keep])
+    _close(rows[0], _want(x, w, b, t, 0.0)["rows"], "rows")
+
+
+@pytest.mark.parametrize("drop", [10.0, 28.0, 60.0])
+def test_rare_tokens_keep_their_bits(cuda, drop):
+    """Tokens of small probabilities whose block of 128 has no target: their rows of dW are as exact, relative to the
+    terms they sum, as any others. (One bound for the entries of G, relative to the probability.)"""
+    P, D, V = 200, 48, 400
+    x, w, b, t = _make(P, D, V, seed=25)
+    t %= 128
+    b[128:] -= drop
+    _, grads = _run(x, w, b, t)
+    X, W, B = (v.double() for v in (x, w, b))
+    l = X @ W.t() + B
+    top = l.amax(1, keepdim=True)
+    p = torch.softmax(l, 1)[:, 128:]
+    worst = (g(D) * (X.abs() @ W.abs().t()) + 2 * E * l.abs()).amax(1, keepdim=True)
+    worst = worst + 2.0 ** -39 * (float(X.abs().max()) * W.abs().sum(1).max() + float(W.abs().max()) * X.abs().sum(1, keepdim=True))
+    ep = 2 * worst + (V / 256 + 24) * E + 8 * E + 2 * E * (l - top).abs()[:, 128:]
+    terms = p.t() @ X.abs()
+    err = (p * ep).t() @ X.abs() + (g(P) + 6 * E) * terms
+    err += 2.0 ** -39 * (float(X.abs().max()) * p.sum(0)[:, None] + float(p.max()) * X.abs().sum(0))
+    want = p.t() @ X / P
+    assert torch.all((grads["w"][128:].double() - want).abs() <= err / P)
+    assert float((err / P).max()) < 1e-4 * float(want.abs().max())
+
+
 @pytest.mark.parametrize("P,D,V", [(40, 32, 64), (64, 33, 50), (7, 2, 20), (300, 1, 9), (2, 3, 5)])
 @pytest.mark.parametrize("value", [1e6, 1e20, 3e38])
 def test_rows_that_do_not_count_may_hold_large_values(cuda, P, D, V, value):
