@@ -359,6 +359,19 @@ def test_a_large_row_costs_the_others_no_bits(cuda):
     _close(rows[0], _want(x, w, b, t, 0.0)["rows"], "rows")
 
 
+@pytest.mark.parametrize("k", [100, -100, 60, -60])
+def test_operands_of_extreme_size(cuda, k):
+    """x 2^k and w 2^-k have the same logits: the same loss to the bit, dx and dw with their powers of two, also where
+    the scales of two blocks together leave the range of one fp32 factor."""
+    x, w, b, t = _make(300, 70, 260, seed=26)
+    norm = torch.tensor([1.0], device="cuda")
+    want = _run(x, w, b, t, grad_norm=norm)
+    got = _run(x * 2.0 ** k, w * 2.0 ** -k, b, t, grad_norm=norm)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1]["b"], want[1]["b"])
+    assert torch.equal(got[1]["x"].double() * 2.0 ** k, want[1]["x"].double())
+    assert torch.equal(got[1]["w"].double() * 2.0 ** -k, want[1]["w"].double())
+
+
 @pytest.mark.parametrize("drop", [10.0, 28.0, 60.0])
 def test_rare_tokens_keep_their_bits(cuda, drop):
     """Tokens of small probabilities whose block of 128 has no target: their rows of dW are as exact, relative to the

@@ -253,6 +253,20 @@ def test_parameter_groups(cuda):
         assert torch.equal(vals["gate"].grad[spans], grads["gate"])
 
 
+@pytest.mark.parametrize("R,D", [(1, 24), (9, 33), (6, 512), (5, 4100)])
+def test_one_value_in_every_place_of_its_shape(cuda, R, D):
+    """x, the branch and a gate per token are one Value: it receives the sum of the three gradients."""
+    ops, dh, dy = _make(R, D, 1, "rms", False, "token", seed=34)
+    ops["branch"] = ops["gate"] = ops["x"]
+    apart = _run({k: v.clone() for k, v in ops.items()}, dh, dy, "rms", 0.5)[2]
+    x, gamma = Value.leaf(ops["x"], True), Value.leaf(ops["gamma"], True)
+    h, y = F.residual_norm(x, x, gamma, None, EPS, kind="rms", gate=x, scale=0.5)
+    backward((h, y), (dh, dy))
+    parts = [apart[k].double() for k in ("x", "branch", "gate")]
+    assert torch.all((x.grad.double() - sum(parts)).abs() <= 2 * E * sum(v.abs() for v in parts))
+    assert torch.equal(gamma.grad, apart["gamma"])
+
+
 @pytest.mark.parametrize("roots", ["y", "hy", "h", "consumer"])
 def test_no_partial_gradient_is_left_on_h(cuda, roots):
     """h's whole gradient is never stored: h.grad is None after a pass, and passes over the same graph repeat."""
