@@ -3,7 +3,9 @@
 //
 // The tensors' sizes and pointers travel in the kernel's parameters (no table in device memory, nothing
 // to upload, nothing two captured graphs could share): kernel parameter blocks hold up to 32764 bytes.
-// Every CTA takes one chunk of one tensor; it finds the tensor by bisecting the chunks' running count.
+// Every CTA takes one chunk of one tensor; it finds the tensor by bisecting the chunks' running count, whose
+// dependent loads a CTA of 1024 elements (8 bits) feels: 203 M elements in one tensor take 601 us, in 56 tensors
+// 676, in 133 702 (32 bits, chunks of 4096: 842, 847 and 855).
 //
 // 32 bits: the element operations and their order are adamw_kernel's (ops_elementwise.cu), so the
 // results are bitwise those of one nnb_adamw_step per tensor. It moves 28 bytes per element and is
@@ -13,7 +15,7 @@
 // block-wise quantization, 2022), with a code chosen for arithmetic instead of a table: 256 consecutive
 // elements share one fp32 unit u, and the code k (signed for m, unsigned for the root r of v) stands
 // for sign(k) k^2 u, u = max / 127^2 or max / 255^2 over the block. Square-law codes are fine near the
-// block's largest value (half a step is 0.4 % for m, 0.2 % for r) and reach down to u; a value is
+// block's largest value (half a step is 0.8 % for m, 0.4 % for r) and reach down to u; a value is
 // stored as the nearest one that a code stands for, a root above zero never as zero (an update divides
 // by it). The root is stored instead of v because its range is half of v's in powers of ten. Per
 // element the step moves 16 bytes instead of 28.
@@ -257,8 +259,8 @@ __device__ __forceinline__ void step_block(Block8& b, const Scalars& s, bool vec
 }
 
 // One block per warp, in small CTAs: 56 registers leave 36 warps on an SM, whose loads cover HBM's
-// latency and each other's arithmetic (about 80 instructions per element, most of what the issue
-// slots give in the time HBM needs). 2^27 elements: 398 us, 5.4 TB/s, 0.82 of the measured copy rate; with an
+// latency and each other's arithmetic (about 95 instructions per element, four fifths of the issue
+// slots). 2^27 elements: 398 us, 5.4 TB/s, 0.82 of the measured copy rate; with an
 // approximate reciprocal in place of the update's division 371 us, but the update is held to the 32-bit
 // step's roundings. Measured against it: 64 registers and 32 warps 404 us; CTAs of 256 threads 4 to 6 %
 // slower; several blocks per warp, even with the next block's loads issued ahead, 8 to 130 % slower (the

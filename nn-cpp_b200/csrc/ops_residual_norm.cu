@@ -15,14 +15,21 @@
 //   dgate = sum over its rows of scale p dt;   dp = scale gate dt;   dbranch = dp, or post's backward
 //   dgamma = sum dy hat, dbeta = sum dy, and the same of dp for post's parameters.
 //
-// Both directions read every row once and keep it in registers: 16 bytes per element forward, 20 to 24
-// backward, so HBM bounds them (32768 x 512 layer: 39 us and 52 us, 6.9 and 6.5 TB/s; 8190 x 2048 rms with post
-// and gate: 43 and 73). T threads share a row (a power of two of warps, so that a thread holds
-// few columns); rows whose length is a multiple of 4 and whose buffers are 16-byte aligned move as
-// float4. In the backward each T-thread slot walks a run of consecutive rows and keeps its columns'
-// parameter sums in registers; the CTA's slots are summed in shared memory, and a second kernel sums
-// the CTAs. Run lengths and orders depend on the rows per parameter group, the gate's span and D only,
-// never on the grid or the GPU, so the sums are bitwise reproducible. All sums are fp32.
+// Both directions read every row once and, for rows of up to 4096 columns, keep it in registers: 16 bytes per
+// element forward, 20 to 24 backward, so HBM bounds them (with the parameter sums' kernel, about 8 us, in the
+// second figure: 32768 x 512 layer 41 us and 64 us, floors 41 and 51; 8190 x 2048 rms with post and gate 43
+// and 74, floors 41 and 61). Above 4096 columns a row's 1024 threads have 64 registers each, too few for the
+// backward's five sums and four operands per column, and it spills: 2048 x 8192 layer 43 + 64 us, with post and
+// gate 56 + 131; 1024 x 16384 48 + 87 us and 69 + 303. Rows that do not move as float4 pay for 4-byte accesses
+// (16384 x 1001 layer 45 + 81 us, with post and gate 63 + 138), rows of up to 128 columns for idle lanes
+// (262144 x 64 rms 53 + 87, 131072 x 128 layer with post and gate 48 + 94).
+//
+// T threads share a row (a power of two of warps, so that a thread holds few columns); rows whose length is a
+// multiple of 4 and whose buffers are 16-byte aligned move as float4. In the backward each T-thread slot walks
+// a run of consecutive rows and keeps its columns' parameter sums in registers; the CTA's slots are summed in
+// shared memory, and a second kernel sums the CTAs. Run lengths and orders depend on the rows per parameter
+// group, the gate's span and D only, never on the grid or the GPU, so the sums are bitwise reproducible. All
+// sums are fp32.
 #include <initializer_list>
 
 #include "nnb_ops.h"

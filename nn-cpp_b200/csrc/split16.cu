@@ -4,15 +4,15 @@
 //   warp 0     TMA producer: a stage holds a 32-deep k-block, A 128 and B 256 rows (or columns), hi[, lo];
 //   warp 1     MMA issuer: kind::f16 128 x 256 x 16 into two TMEM accumulators in turn, one accumulator per
 //              chunk of 128 terms (3 x 8 MMAs);
-//   warps 4-11 epilogue: add each finished chunk, scaled back, into registers (128 columns per thread) while the tensor
-//              core works on the next, then store or reduce.
+//   warps 4-11 epilogue: add each finished chunk, scaled back, into registers (128 columns per thread) while
+//              the tensor core works on the next, then store or reduce.
 // The 384 threads are launched with 168 registers each; warps 0-3 hand theirs down to 56 and the epilogue
 // takes 224 (4 x 32 x 56 + 8 x 32 x 224 = 384 x 168), which hold the 128 sums.
 // Tensor bound: 3 MMAs per 128 x 256 x 16 step, 1.6 PFLOP/s of fp16 (the measured bf16 burst rate) or 540
-// TFLOP/s of the fp32 product. Measured at 137 GFLOP (32768 x 512 x 4096, each way round): 306 us (450 TFLOP/s,
-// the pipe 71 to 74 % active at a power-capped 1.5 GHz) where the depth is 4096 or more, 385 us with the
+// TFLOP/s of the fp32 product. Measured at 137 GFLOP (32768 x 512 x 4096, each way round): 300 to 313 us (450
+// TFLOP/s, the pipe 73 to 75 % active at a power-capped 1.5 GHz) where the depth is 4096 or more, 366 us with the
 // depth of 512, whose epilogue writes 128 KB of logits and takes 128 exponentials per thread for every
-// four chunks; 570 us for 275 GFLOP (482 TFLOP/s) with the statistics alone.
+// four chunks; 548 us for 275 GFLOP (502 TFLOP/s) with the statistics alone.
 // The tile: 128 x 256 and two accumulators fill TMEM, and 128 sums per thread fill the registers. A chunk
 // of 256 or 512 terms instead of 128 gains 5 % and costs 2 and 4 times the error.
 #include <algorithm>
@@ -52,7 +52,8 @@ struct PackJobs {
 
 // One block of 128 x 128 per CTA, held in registers: 16 float4 per thread (or single floats), a warp on the 128
 // columns of a row; its largest magnitude; then 8 bytes of hi and of lo out per float4. HBM bound: 4 bytes in and
-// 4 out per value (131072 x 512: 97 us, 5.5 TB/s; a range pass over the matrix and a pack after it took 148).
+// 4 out per value (131072 x 512: 97 us, 5.5 TB/s; a range pass over the matrix and a pack after it took 148; a CTA's loads and
+// stores do not overlap, only those of the SM's two CTAs).
 __global__ void __launch_bounds__(256, 2) pack_kernel(const PackJobs jobs) {
 	__shared__ unsigned tops[8];
 	const bool second = (int)blockIdx.x >= jobs.first;

@@ -910,8 +910,9 @@ def linear_cross_entropy(x: Value, weight: Value, bias: Value | None, targets: t
     the targets that are not ignore_index, label smoothing and grad_norm as sequence_cross_entropy's.
 
     The rows go through in pieces; where a gradient is needed it is computed with the loss, from the same
-    logits, and the backward only scales it (nnb_linear_ce_fwd, include/nnb.h). For inputs that need
-    none, see linear_token_losses."""
+    logits, and the backward only scales it (nnb_linear_ce_fwd, include/nnb.h): a second copy of the gradients,
+    per parameter group, is kept until the graph goes, also for a loss that is only read. For inputs that need
+    none, see linear_token_losses. The backward runs in the parameter groups of the forward."""
     _check_grad_norm(grad_norm)
     P, D, V = _linear_ce_args("linear_cross_entropy", x, weight, bias, targets)
     parents = (x, weight) if bias is None else (x, weight, bias)
