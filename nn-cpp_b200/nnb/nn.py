@@ -665,12 +665,12 @@ class AdamW:
             self.t += 1
             return
         s = F._s()
+        w = _addresses("AdamW", [p.data for p in self.params], self._sizes)
+        g = _addresses("AdamW", [p.grad for p in self.params], self._sizes)
         for p in self.params:
             if p.grad_fresh:     # nothing reached this parameter: its gradient is all zeros
                 check(lib().nnb_fill(s, p.grad.numel(), 0.0, p.grad.data_ptr()))
                 p.grad_fresh = False
-        w = _addresses("AdamW", [p.data for p in self.params], self._sizes)
-        g = _addresses("AdamW", [p.grad for p in self.params], self._sizes)
         update = lib().nnb_adamw_multi_step if self.state_bits == 32 else lib().nnb_adamw8_multi_step
         scalars = (self.lr, self.beta1, self.beta2, self.eps, self.weight_decay)
         self.t += 1

@@ -195,6 +195,21 @@ def test_8bit_update_is_rounded_like_the_32bit_one(cuda, n):
     assert np.array_equal(p.data.cpu().numpy().view(np.int32), want.view(np.int32))
 
 
+def test_a_refused_step_writes_nothing(cuda):
+    """A gradient that nothing reached stands for zeros; where the step is refused, no buffer is filled with them."""
+    params = _params([40, 30], 12)
+    opt = nn.AdamW(params, **HYPER)
+    flat = torch.arange(200.0, device="cuda")
+    for grad in (flat.view(4, 50)[:, :10], flat[:50], flat[:80:2]):
+        params[0].grad, params[0].grad_fresh = grad, True
+        with pytest.raises(ValueError):
+            opt.step()
+        assert torch.equal(flat, torch.arange(200.0, device="cuda")) and params[0].grad_fresh and opt.t == 0
+    params[0].grad = flat[:40]
+    opt.step()
+    assert torch.equal(flat[:40], torch.zeros(40, device="cuda")) and float(flat[40]) == 40.0
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_parameters_that_share_memory(cuda, bits):
     """Slices of one buffer that overlap are updated one after the other in the list's order, each with its own
